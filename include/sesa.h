@@ -67,6 +67,9 @@ extern "C" {
                              QKV / FF Linears single fp16 pass; the rest bf16x3                           */
 #define SESA_PREC_F16MIX 4 /* MDX23C: per-level plan of the T >= 32 TFC 3x3 convs (sesa_mdx23c_set_f16_plan);
                               HTDemucs: fp16 attention + convs; SCNet: fp16 token GEMMs */
+#define SESA_PREC_I8 5    /* BS- / Mel-Band-Roformer: the QKV / out / FF Linears on 8-bit integers (one scale per
+                             token and per output channel), fp16 attention; the rest as SESA_PREC_F16.  Opt-in: about
+                             1 % relative error, outside the 1e-4 RMS gate                                */
 
 int sesa_version(void);
 const char* sesa_last_error(void);
@@ -285,6 +288,139 @@ size_t sesa_htdemucs_workspace_size(const sesa_htdemucs* m, int batch);
 int sesa_htdemucs_forward(sesa_htdemucs* m, const float* x, int batch, float* out, void* workspace,
                           size_t workspace_bytes, void* stream);
 int sesa_htdemucs_destroy(sesa_htdemucs* m);
+
+/* ---------------------------------------------------------------------------------------
+ * Transformer operators in the 16- and 8-bit types (no reference counterpart; the Roformers' SESA_PREC_I8 forward
+ * is built from them).  Rows are contiguous in their last dimension; every other stride (`*_ld`, `*_t`, ...) counts
+ * elements of that tensor and may be any value that keeps the rows apart.  No workspace; a call with no rows
+ * returns SESA_OK without a launch.  Forward only.
+ */
+#define SESA_DTYPE_F32 0
+#define SESA_DTYPE_F16 1
+#define SESA_DTYPE_BF16 2
+
+#define SESA_ACT_NONE 0
+#define SESA_ACT_GELU 1 /* erf form */
+#define SESA_ACT_TANH 2
+#define SESA_ACT_RELU 3
+
+/* Linear layer on 8-bit integers with one scale per token and one per output channel:
+ *   out[m, n] = act( x_scale[m] * w_scale[n] * sum_k x[m, k] * w[n, k] + bias[n] )
+ * x [m, k] and w [n, k] int8, the sum in 32-bit integers (exact for k <= 131071, the largest accepted), the scales,
+ * bias (nullable) and epilogue in fp32, out rounded once to out_dtype.  A scale that is NaN makes its row / column NaN.
+ */
+int sesa_linear_i8(const int8_t* x, int64_t x_ld, const float* x_scale, const int8_t* w, int64_t w_ld,
+                   const float* w_scale, const float* bias, int act, int64_t m, int n, int k, void* out, int out_dtype,
+                   int64_t o_ld, void* stream);
+
+#define SESA_NORM_NONE 0
+#define SESA_NORM_RMS 1   /* v * rsqrt(mean(v^2) + eps) * weight (+ bias)                                   */
+#define SESA_NORM_LAYER 2 /* (v - mean(v)) * rsqrt(mean((v - mean(v))^2) + eps) * weight + bias             */
+
+#define SESA_GATE_NONE 0  /* the gate itself multiplies */
+#define SESA_GATE_SIGMOID 1
+#define SESA_GATE_SILU 2
+#define SESA_GATE_TANH 3
+
+/* The seam between two transformer blocks in one pass over the rows:
+ *   y = residual + scale * gate_act(gate) * post_norm(x)        (the block's output joins the residual stream)
+ *   n = pre_norm(y)                                              (the next block's input)
+ * residual, scale, gate and the norms are optional; statistics and everything between the loads and the one
+ * rounding of y and of n are fp32 (n comes from the unrounded y).  With q instead of n the rows leave in 8 bits:
+ *   q_scale = max |n| / 127 over the row, q = round-half-even(n / q_scale)
+ * (an all-zero row: scale 0, q 0; a row holding a NaN or an infinity: scale NaN, q 0).
+ * y may be residual (same ld): in place.  No other operands may overlap.  dim <= 32768.
+ */
+typedef struct sesa_norm_args {
+  int64_t rows;
+  int dim;
+  int x_dtype;                /* of x, gate and n                                                        */
+  int r_dtype;                /* of residual and y: x_dtype or SESA_DTYPE_F32                            */
+  const void* x;
+  int64_t x_ld;
+  const void* residual;       /* nullable: 0                                                             */
+  int64_t r_ld;
+  const void* gate;           /* nullable: 1; gate row of row r is r / rows_per_gate                     */
+  int64_t gate_ld;
+  int64_t rows_per_gate;
+  int gate_act;               /* SESA_GATE_*                                                             */
+  int post;                   /* SESA_NORM_* of x                                                        */
+  const float* post_weight;   /* [dim] fp32, nullable: 1 (also the other parameter vectors)              */
+  const float* post_bias;     /* nullable: 0                                                             */
+  const float* scale;         /* nullable: 1                                                             */
+  int pre;                    /* SESA_NORM_* of y                                                        */
+  const float* pre_weight;
+  const float* pre_bias;
+  float eps;
+  void* y;                    /* nullable: not written                                                   */
+  int64_t y_ld;
+  void* n;                    /* nullable                                                                */
+  int64_t n_ld;
+  int8_t* q;                  /* nullable; at most one of n and q, at least one of y, n and q            */
+  int64_t q_ld;
+  float* q_scale;             /* [rows], with q                                                          */
+} sesa_norm_args;
+
+int sesa_norm_residual(const sesa_norm_args* args, void* stream);
+
+#define SESA_ROPE_HALVES 0 /* pair i of a head = elements (i, i + P), P = sum of the sections */
+#define SESA_ROPE_PAIRS 1  /* pair i of a head = elements (2 i, 2 i + 1)                      */
+
+/* Rotary positions with several axes: sections[a] consecutive pairs of every head turn with axis a,
+ *   (u, v) -> (u cos t - v sin t, u sin t + v cos t),  t = positions[token, a] * freqs[pair]
+ * (freqs in radians per position; the angle is reduced exactly for any integer position, the rotation is fp32).
+ * Elements from 2 P on pass through.  One or two tensors of the same tokens (q and k); out may be x with its strides.
+ */
+typedef struct sesa_rope_tensor {
+  const void* x;              /* [tokens][heads][head_dim], strides x_t, x_h                             */
+  int64_t x_t, x_h;
+  void* out;
+  int64_t o_t, o_h;
+  int heads;
+} sesa_rope_tensor;
+
+typedef struct sesa_rope_args {
+  int64_t tokens;
+  int head_dim, dtype, layout;
+  int n_axes;                 /* 1..4                                                                    */
+  int sections[4];            /* pairs per axis, >= 0; 2 * their sum in [2, head_dim]                    */
+  const void* positions;      /* [tokens][n_axes] int32, or int64 with positions_i64                     */
+  int64_t positions_ld;
+  int positions_i64;
+  const float* freqs;         /* [P] fp32                                                                */
+  int n_tensors;              /* 1 or 2                                                                  */
+  sesa_rope_tensor t[2];
+} sesa_rope_args;
+
+int sesa_rope_axes(const sesa_rope_args* args, void* stream);
+
+/* Softmax attention within each sequence of a packed run of tokens, grouped heads:
+ *   out[i] = sigmoid(gate[i]) * sum_j softmax_j(scale * q[i] . k[j]) v[j],  j over i's own sequence (causal: j <= i)
+ * Sequence s is tokens cu_seqlens[s] .. cu_seqlens[s + 1] - 1 (device int32 [n_seq + 1], non-decreasing; values
+ * are held to [0, tokens] and to that order by the kernel); cu_seqlens NULL: n_seq sequences of tokens / n_seq.
+ * Tokens before cu_seqlens[0] and from cu_seqlens[n_seq] on belong to no sequence: their rows of out are left as
+ * they were, or set to 0 with zero_rest.  `lanes` runs of the same lengths lie side by side (strides *_l).
+ * head_dim a multiple of 8, 8..128; heads a multiple of kv_heads; fp16 or bf16.  Scores, softmax statistics and
+ * sums fp32; the probabilities are rounded once to the type for the product with v.  A masked key contributes
+ * nothing, whatever its k and v hold.  out may not overlap the inputs.
+ */
+typedef struct sesa_attn_args {
+  int64_t tokens;
+  int lanes, heads, kv_heads, head_dim, dtype;
+  const void *q, *k, *v;      /* [tokens][lanes][heads | kv_heads][head_dim]                             */
+  int64_t q_t, q_l, q_h, k_t, k_l, k_h, v_t, v_l, v_h;
+  const int32_t* cu_seqlens;
+  int n_seq;
+  int causal;
+  float scale;
+  const void* gate;           /* nullable; logits [tokens][lanes][heads], strides g_*                    */
+  int64_t g_t, g_l, g_h;
+  void* out;                  /* [tokens][lanes][heads][head_dim], strides o_*                           */
+  int64_t o_t, o_l, o_h;
+  int zero_rest;
+} sesa_attn_args;
+
+int sesa_attention_packed(const sesa_attn_args* args, void* stream);
 
 /* ---------------------------------------------------------------------------------------
  * Ensemble blend (ensemble.py:172-407, AudioEnsembleEngine.process_waveform / process_spectral /

@@ -1,0 +1,298 @@
+// sesa_attention_packed: softmax attention within each sequence of a packed run, grouped heads, optional head gate.
+//
+// One pass over the keys with a running maximum and sum (fp32).  S^T = K Q^T on v_mfma_*_32x32x16: a lane then holds
+// one query's scores, so the row statistics need a single exchange (the two lane halves), and the same registers,
+// rounded to the type, are the second operand of O^T += V^T P^T; V^T comes from LDS by transposing 16-bit reads.
+#include "sesa_tokens.hpp"
+
+namespace sesa {
+namespace {
+
+constexpr int kKeys = 64;   // keys per block
+
+template <class T>
+__device__ __forceinline__ f32x16 mfma16(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (std::is_same<T, f16>::value)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
+                                                   0);
+}
+
+// Region i of the run: i = 0 the tokens before the first sequence, 1 .. n_seq the sequences, n_seq + 1 the rest.
+__device__ __forceinline__ int64_t bound(const sesa_attn_args& a, int i) {
+  if (i == 0) return 0;
+  if (i == a.n_seq + 2) return a.tokens;
+  if (!a.cu_seqlens) return (int64_t)(i - 1) * (a.tokens / a.n_seq);
+  const int64_t c = a.cu_seqlens[i - 1];
+  return c < 0 ? 0 : (c > a.tokens ? a.tokens : c);
+}
+
+// Query tiles: region i owns the slots bound(i) / BQ + i .. bound(i + 1) / BQ + i -- at least as many as its tiles of BQ
+// tokens -- so a workgroup finds its tile from the boundaries alone (64 of them compared at a time), and the grid needs
+// no count from the device.  The slots left over (less than one a region) end at once.
+template <int BQ>
+__device__ __forceinline__ bool find_tile(const sesa_attn_args& a, int slot, int* region, int* q0, int* start, int* end) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, hi = a.n_seq + 2;
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 63) / 64, i = lo + lane * step;
+    const bool at = i < hi && bound(a, i) / BQ + i <= slot;
+    const int c = max(1, (int)__popcll(__ballot(at)));
+    lo += (c - 1) * step;
+    hi = min(hi, lo + step);
+  }
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  const int64_t b = bound(a, lo), e = bound(a, lo + 1), q = b + (slot - (b / BQ + lo)) * (int64_t)BQ;
+  *region = lo;
+  *start = (int)b;
+  *end = (int)e;
+  *q0 = (int)q;
+  return q >= b && q < e;
+}
+
+template <class T, int D, int NW>
+__global__ void __launch_bounds__(NW * 64, 2) attn_packed_kernel(sesa_attn_args a, int n_slots) {
+  constexpr int BQ = NW * 32, NTH = NW * 64, ROW = D * 2, IMG = kKeys * ROW, CH = D / 8, IT = kKeys * CH / NTH;
+  constexpr float kLog2e = 1.4426950408889634f;
+  __shared__ __attribute__((aligned(16))) char smem[4 * IMG];   // [stage][K, V], rows of D elements
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l32 = lane & 31, hl = lane >> 5;
+  const int group = a.heads / a.kv_heads;
+  // a die's workgroups: consecutive query heads and tiles of one (lane, key head), so its L2 holds that head's K and V
+  int t = die_tile(blockIdx.x, gridDim.x);
+  const int gi = t % group;
+  t /= group;
+  const int slot = n_slots - 1 - t % n_slots;   // causal: the longest tiles first
+  t /= n_slots;
+  const int kh = t % a.kv_heads, ln = t / a.kv_heads;
+  const int head = kh * group + gi;
+  int region, q0, start, end;
+  if (!find_tile<BQ>(a, slot, &region, &q0, &start, &end)) return;
+  const int64_t q_pos = (int64_t)q0 + wave * 32 + l32;
+  const bool q_ok = q_pos < end;
+  T* out = reinterpret_cast<T*>(a.out) + q_pos * a.o_t + ln * a.o_l + head * a.o_h;
+  if (region == 0 || region == a.n_seq + 1) {
+    if (a.zero_rest && q_ok)
+      for (int d = 8 * hl; d < a.head_dim; d += 16) store16(out + d, u32x4{0u, 0u, 0u, 0u});
+    return;
+  }
+  const int hd = a.head_dim;
+  const T* kp = reinterpret_cast<const T*>(a.k) + ln * a.k_l + kh * a.k_h;
+  const T* vp = reinterpret_cast<const T*>(a.v) + ln * a.v_l + kh * a.v_h;
+
+  u32x4 qf[D / 16];
+  {
+    const T* qp = reinterpret_cast<const T*>(a.q) + q_pos * a.q_t + ln * a.q_l + head * a.q_h;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+      const int d = 16 * ks + 8 * hl;
+      qf[ks] = q_ok && d < hd ? load16(qp + d) : u32x4{0u, 0u, 0u, 0u};
+    }
+  }
+  f32x16 o[D / 32];
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[db][r] = 0.f;
+  float m_run = -INFINITY, l_run = 0.f;   // running maximum (of the raw scores) and sum
+  const float c = a.scale * kLog2e;
+
+  auto swz = [](int row, int chunk) { return row * ROW + ((chunk ^ (row & 7)) << 4); };
+  u32x4 kreg[IT], vreg[IT];
+  auto load_block = [&](int kb) {
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      const int e = tid + i * NTH, key = e / CH, d = e % CH * 8;
+      const int64_t p = (int64_t)start + kb * kKeys + key;
+      const bool ok = p < end && d < hd;   // zeros behind the sequence and behind head_dim
+      kreg[i] = ok ? load16(kp + p * a.k_t + d) : u32x4{0u, 0u, 0u, 0u};
+      vreg[i] = ok ? load16(vp + p * a.v_t + d) : u32x4{0u, 0u, 0u, 0u};
+    }
+  };
+  auto store_block = [&](char* stage) {
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      const int e = tid + i * NTH, off = swz(e / CH, e % CH);
+      *reinterpret_cast<u32x4*>(stage + off) = kreg[i];
+      *reinterpret_cast<u32x4*>(stage + IMG + off) = vreg[i];
+    }
+  };
+  // V^T fragment (d-block db, keys 16 ks ..): lane half hl gets the keys 4 hl .. + 3 and 8 + 4 hl .. + 3 of its step,
+  // the order in which the score registers hold them
+  const int tg = lane >> 4, ti = lane & 15;
+  auto vt = [&](const char* V, int ks, int db) -> u32x4 {
+    typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+    const int d = db * 32 + 16 * (tg & 1) + 4 * (ti & 3), key = 16 * ks + 4 * (tg >> 1) + (ti >> 2);
+    const bf16x4 t0 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
+        (__attribute__((address_space(3))) bf16x4*)(V + swz(key, d >> 3) + ((d & 7) << 1)));
+    const bf16x4 t1 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
+        (__attribute__((address_space(3))) bf16x4*)(V + swz(key + 8, d >> 3) + ((d & 7) << 1)));
+    return __builtin_bit_cast(u32x4, __builtin_shufflevector(t0, t1, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+
+  const int last = a.causal ? min(end, q0 + BQ) : end;   // keys from here on reach no query of the tile
+  const int n_blocks = (last - start + kKeys - 1) / kKeys;
+  load_block(0);
+  store_block(smem);
+  if (n_blocks > 1) load_block(1);
+  sesa_sync();
+  for (int kb = 0; kb < n_blocks; ++kb) {
+    const char* K = smem + (kb & 1) * 2 * IMG;
+    const char* V = K + IMG;
+    f32x16 s[2];
+#pragma unroll
+    for (int rb = 0; rb < 2; ++rb) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[rb][r] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        const u32x4 kf = *reinterpret_cast<const u32x4*>(K + swz(rb * 32 + l32, 2 * ks + hl));
+        s[rb] = mfma16<T>(kf, qf[ks], s[rb]);
+      }
+    }
+    // block kb + 1 (loaded an iteration ago) into the other stage, whose last reads the barrier below has closed
+    if (kb + 1 < n_blocks) {
+      store_block(smem + ((kb + 1) & 1) * 2 * IMG);
+      if (kb + 2 < n_blocks) load_block(kb + 2);
+    }
+    const int key0 = start + kb * kKeys;
+    const bool diagonal = a.causal && key0 + kKeys - 1 > q0 + wave * 32;
+    if (diagonal || key0 + kKeys > end) {
+      const int64_t lim = a.causal ? min((int64_t)end - 1, q_pos) : (int64_t)end - 1;   // last key this query sees
+#pragma unroll
+      for (int rb = 0; rb < 2; ++rb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int key = key0 + rb * 32 + (r & 3) + 8 * (r >> 2) + 4 * hl;
+          if (key > lim) s[rb][r] = -INFINITY;
+        }
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int rb = 0; rb < 2; ++rb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[rb][r]);
+    top = fmaxf(top, __shfl_xor(top, 32));
+    // The running maximum moves only when a block exceeds it by more than 2^8 in the exponential (P stays <= 256, in
+    // range for fp16), so most blocks leave O alone.  Both halves of a query hold the same values, so they agree.
+    if ((top - m_run) * c > 8.f || (m_run == -INFINITY && top > -INFINITY)) {
+      const float alpha = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_run - top) * c);
+      l_run *= alpha;
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
+      m_run = top;
+    }
+    const float mc = m_run == -INFINITY ? 0.f : m_run * c;   // (no finite score so far: every P is exp(-inf) = 0)
+    float sum = 0.f;
+#pragma unroll
+    for (int rb = 0; rb < 2; ++rb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float p = __builtin_amdgcn_exp2f(fmaf(s[rb][r], c, -mc));
+        s[rb][r] = p;
+        sum += p;
+      }
+    l_run += sum + __shfl_xor(sum, 32);
+    // A diagonal block multiplies probabilities of 0 with keys behind the query: harmless for finite v, but 0 * inf is
+    // NaN, so look for non-finite v there (exponent all ones) and take that block element by element if there is one.
+    uint32_t bad = 0;
+    constexpr uint32_t kExp = std::is_same<T, f16>::value ? 0x7c007c00u : 0x7f807f80u;
+    constexpr uint32_t kOne = std::is_same<T, f16>::value ? 0x04000400u : 0x00800080u;
+    if (diagonal) {
+      for (int e = lane; e < IMG / 16; e += 64) {
+        const u32x4 w = *reinterpret_cast<const u32x4*>(V + e * 16);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) bad |= (w[q] & kExp) + kOne;
+      }
+    }
+    if (__ballot((bad & 0x80008000u) != 0)) {
+#pragma unroll
+      for (int rb = 0; rb < 2; ++rb)
+#pragma unroll 1
+        for (int r = 0; r < 16; ++r) {
+          const float mine = s[rb][r];
+#pragma unroll 1
+          for (int half = 0; half < 2; ++half) {
+            const float p = __shfl(mine, l32 + 32 * half);
+            const int key = rb * 32 + (r & 3) + 8 * (r >> 2) + 4 * half;
+            if (key0 + key > q_pos) continue;
+#pragma unroll
+            for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+              for (int q = 0; q < 16; ++q) {
+                const int d = db * 32 + 8 * (q >> 2) + 4 * hl + (q & 3);
+                o[db][q] = fmaf(p, (float)*reinterpret_cast<const T*>(V + swz(key, d >> 3) + ((d & 7) << 1)), o[db][q]);
+              }
+          }
+        }
+    } else {
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        const f32x16& sv = s[ks >> 1];
+        const int r0 = 8 * (ks & 1);
+        const u32x4 pf = {pack2t<T>(sv[r0], sv[r0 + 1]), pack2t<T>(sv[r0 + 2], sv[r0 + 3]),
+                          pack2t<T>(sv[r0 + 4], sv[r0 + 5]), pack2t<T>(sv[r0 + 6], sv[r0 + 7])};
+#pragma unroll
+        for (int db = 0; db < D / 32; ++db) o[db] = mfma16<T>(vt(V, ks, db), pf, o[db]);
+      }
+    }
+    sesa_sync();
+  }
+
+  if (!q_ok) return;
+  float scale = 1.f / l_run;
+  if (a.gate) scale *= sigmoid_f((float)reinterpret_cast<const T*>(a.gate)[q_pos * a.g_t + ln * a.g_l + head * a.g_h]);
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const int d = db * 32 + 8 * b + 4 * hl;
+      if (d >= hd) continue;
+      struct __attribute__((packed)) B8 { uint32_t a, b; };
+      *reinterpret_cast<B8*>(out + d) = B8{pack2t<T>(o[db][4 * b] * scale, o[db][4 * b + 1] * scale),
+                                           pack2t<T>(o[db][4 * b + 2] * scale, o[db][4 * b + 3] * scale)};
+    }
+}
+
+template <class T>
+int launch_attn(const sesa_attn_args& a, hipStream_t st) {
+  constexpr int NW = 4;
+  const int64_t n_slots = a.tokens / (NW * 32) + a.n_seq + 2;
+  const int64_t blocks = n_slots * a.heads * a.lanes;
+  SESA_REQUIRE(blocks < (1ll << 31), SESA_ERR_INVALID, "attention_packed: too many tokens x heads x lanes");
+  if (a.head_dim <= 64)
+    hipLaunchKernelGGL((attn_packed_kernel<T, 64, NW>), dim3((unsigned)blocks), dim3(NW * 64), 0, st, a, (int)n_slots);
+  else
+    hipLaunchKernelGGL((attn_packed_kernel<T, 128, NW>), dim3((unsigned)blocks), dim3(NW * 64), 0, st, a, (int)n_slots);
+  SESA_CHECK_LAUNCH();
+  return SESA_OK;
+}
+
+}  // namespace
+}  // namespace sesa
+
+using namespace sesa;
+
+extern "C" int sesa_attention_packed(const sesa_attn_args* args, void* stream) {
+  clear_error();
+  SESA_REQUIRE(args, SESA_ERR_INVALID, "attention_packed: null arguments");
+  const sesa_attn_args& a = *args;
+  SESA_REQUIRE(a.tokens >= 0 && a.tokens < (1ll << 31) - 1024, SESA_ERR_INVALID, "attention_packed: tokens %lld",
+               (long long)a.tokens);
+  SESA_REQUIRE(a.lanes >= 1 && a.heads >= 1 && a.kv_heads >= 1 && a.heads % a.kv_heads == 0, SESA_ERR_INVALID,
+               "attention_packed: lanes %d, heads %d, kv_heads %d", a.lanes, a.heads, a.kv_heads);
+  SESA_REQUIRE(a.head_dim >= 8 && a.head_dim <= 128 && a.head_dim % 8 == 0, SESA_ERR_INVALID,
+               "attention_packed: head_dim %d (a multiple of 8, 8..128)", a.head_dim);
+  SESA_REQUIRE(a.dtype == SESA_DTYPE_F16 || a.dtype == SESA_DTYPE_BF16, SESA_ERR_INVALID, "attention_packed: dtype %d",
+               a.dtype);
+  SESA_REQUIRE(a.n_seq >= 1 && a.n_seq < (1 << 30), SESA_ERR_INVALID, "attention_packed: n_seq %d", a.n_seq);
+  SESA_REQUIRE(a.cu_seqlens || a.tokens % a.n_seq == 0, SESA_ERR_INVALID,
+               "attention_packed: %lld tokens are not %d sequences of one length", (long long)a.tokens, a.n_seq);
+  SESA_REQUIRE(a.scale > 0.f && a.scale < INFINITY, SESA_ERR_INVALID, "attention_packed: scale %g", (double)a.scale);
+  if (a.tokens == 0) return SESA_OK;
+  SESA_REQUIRE(a.q && a.k && a.v && a.out, SESA_ERR_INVALID, "attention_packed: null operand");
+  hipStream_t st = as_stream(stream);
+  return a.dtype == SESA_DTYPE_F16 ? launch_attn<f16>(a, st) : launch_attn<__bf16>(a, st);
+}

@@ -1,0 +1,102 @@
+// Shared device helpers of the transformer operators (sesa_norm / sesa_rope / sesa_linear_i8 / sesa_attn_packed).
+#pragma once
+#include <hip/hip_runtime.h>
+#include <cmath>
+#include <cstdint>
+
+#include "sesa_common.hpp"
+
+namespace sesa {
+
+typedef _Float16 f16;
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+// 16 bytes at any address: the rows of the public operators start where the caller's strides put them, and gfx950
+// loads and stores a dwordx4 at any byte (one instruction; only the cache lines it touches count).
+struct __attribute__((packed)) Bytes16 {
+  u32x4 v;
+};
+
+__device__ __forceinline__ u32x4 load16(const void* p) { return reinterpret_cast<const Bytes16*>(p)->v; }
+__device__ __forceinline__ void store16(void* p, u32x4 v) { reinterpret_cast<Bytes16*>(p)->v = v; }
+
+// Eight consecutive elements of a row as fp32; `left` = elements of the row from here on (<= 0: none).  Whole groups
+// take vector loads, a row's last partial group goes element by element (zero past its end).
+template <class T>
+__device__ __forceinline__ void load8(const T* p, int left, float (&v)[8]) {
+  if (left >= 8) {
+    if constexpr (sizeof(T) == 4) {
+      // (whole vectors: a bit cast of one vector element reads element 0 whatever the index is)
+      const f32x4 a = __builtin_bit_cast(f32x4, load16(p)), b = __builtin_bit_cast(f32x4, load16(p + 4));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[e] = a[e];
+        v[4 + e] = b[e];
+      }
+    } else {
+      const u32x4 a = load16(p);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[2 * e] = (float)__builtin_bit_cast(T, (uint16_t)(a[e] & 0xffffu));
+        v[2 * e + 1] = (float)__builtin_bit_cast(T, (uint16_t)(a[e] >> 16));
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e < left ? (float)p[e] : 0.f;
+  }
+}
+
+template <class T>
+__device__ __forceinline__ uint32_t pack2t(float a, float b) {
+  return (uint32_t)__builtin_bit_cast(uint16_t, (T)a) | ((uint32_t)__builtin_bit_cast(uint16_t, (T)b) << 16);
+}
+
+template <class T>
+__device__ __forceinline__ void store8(T* p, int left, const float (&v)[8]) {
+  if (left >= 8) {
+    if constexpr (sizeof(T) == 4) {
+      u32x4 a, b;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        a[e] = __builtin_bit_cast(uint32_t, v[e]);
+        b[e] = __builtin_bit_cast(uint32_t, v[4 + e]);
+      }
+      store16(p, a);
+      store16(p + 4, b);
+    } else {
+      store16(p, u32x4{pack2t<T>(v[0], v[1]), pack2t<T>(v[2], v[3]), pack2t<T>(v[4], v[5]), pack2t<T>(v[6], v[7])});
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < left) p[e] = (T)v[e];
+  }
+}
+
+// 16 bytes a lane from anywhere to LDS at the (wave-uniform) base + 16 * lane, counted by vmcnt.  A function of its own:
+// inside a template's lambda the host pass drops the kernel's launch stub over the builtin.
+__device__ __forceinline__ void dma16(const void* src, char* base) {
+  __builtin_amdgcn_global_load_lds(src, (__attribute__((address_space(3))) void*)base, 16, 0, 0);
+}
+
+__device__ __forceinline__ float sigmoid_f(float v) {
+  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * v));
+}
+// tanh(v) = (1 - e) / (1 + e), e = exp(-2 |v|); below 0.09 the odd series to v^7 (next term 2^-26 relative there),
+// where the quotient would cancel.
+__device__ __forceinline__ float tanh_f(float v) {
+  const float z = fabsf(v), e = __builtin_amdgcn_exp2f(-2.f * 1.4426950408889634f * z), s = v * v;
+  const float big = copysignf((1.f - e) * __builtin_amdgcn_rcpf(1.f + e), v);
+  const float small = v * fmaf(s, fmaf(s, fmaf(s, -17.f / 315.f, 2.f / 15.f), -1.f / 3.f), 1.f);
+  return z < 0.09f ? small : big;
+}
+
+// Tile order of a 1-D grid: workgroup b of nb runs on die b % 8, so give each die one contiguous range of tiles (its
+// own L2 then sees neighbouring tiles' operands).
+__device__ __forceinline__ int die_tile(int b, int nb) {
+  const int q = nb >> 3, r = nb & 7, x = b & 7, i = b >> 3;
+  return x * q + min(x, r) + i;
+}
+
+}  // namespace sesa

@@ -15,6 +15,7 @@ SESA_PREC_BF16 = 1
 SESA_PREC_F16W2 = 2
 SESA_PREC_F16 = 3
 SESA_PREC_F16MIX = 4
+SESA_PREC_I8 = 5
 
 
 class SesaMdx23cConfig(ctypes.Structure):
@@ -49,6 +50,35 @@ class SesaHtdemucsConfig(ctypes.Structure):
         "t_norm_first", "t_norm_out", "t_layer_scale", "t_gelu", "t_cross_first")] + [
         (n, ctypes.c_double) for n in ("t_hidden_scale", "freq_emb", "emb_scale", "t_max_period",
                                        "t_weight_pos_embed")] + [("precision", c_int)]
+
+
+class SesaNormArgs(ctypes.Structure):
+    _fields_ = [("rows", c_int64), ("dim", c_int), ("x_dtype", c_int), ("r_dtype", c_int), ("x", c_void_p),
+                ("x_ld", c_int64), ("residual", c_void_p), ("r_ld", c_int64), ("gate", c_void_p), ("gate_ld", c_int64),
+                ("rows_per_gate", c_int64), ("gate_act", c_int), ("post", c_int), ("post_weight", c_void_p),
+                ("post_bias", c_void_p), ("scale", c_void_p), ("pre", c_int), ("pre_weight", c_void_p),
+                ("pre_bias", c_void_p), ("eps", ctypes.c_float), ("y", c_void_p), ("y_ld", c_int64), ("n", c_void_p),
+                ("n_ld", c_int64), ("q", c_void_p), ("q_ld", c_int64), ("q_scale", c_void_p)]
+
+
+class SesaRopeTensor(ctypes.Structure):
+    _fields_ = [("x", c_void_p), ("x_t", c_int64), ("x_h", c_int64), ("out", c_void_p), ("o_t", c_int64),
+                ("o_h", c_int64), ("heads", c_int)]
+
+
+class SesaRopeArgs(ctypes.Structure):
+    _fields_ = [("tokens", c_int64), ("head_dim", c_int), ("dtype", c_int), ("layout", c_int), ("n_axes", c_int),
+                ("sections", c_int * 4), ("positions", c_void_p), ("positions_ld", c_int64), ("positions_i64", c_int),
+                ("freqs", c_void_p), ("n_tensors", c_int), ("t", SesaRopeTensor * 2)]
+
+
+class SesaAttnArgs(ctypes.Structure):
+    _fields_ = [("tokens", c_int64), ("lanes", c_int), ("heads", c_int), ("kv_heads", c_int), ("head_dim", c_int),
+                ("dtype", c_int), ("q", c_void_p), ("k", c_void_p), ("v", c_void_p)] + [
+        (n, c_int64) for n in ("q_t", "q_l", "q_h", "k_t", "k_l", "k_h", "v_t", "v_l", "v_h")] + [
+        ("cu_seqlens", c_void_p), ("n_seq", c_int), ("causal", c_int), ("scale", ctypes.c_float), ("gate", c_void_p),
+        ("g_t", c_int64), ("g_l", c_int64), ("g_h", c_int64), ("out", c_void_p), ("o_t", c_int64), ("o_l", c_int64),
+        ("o_h", c_int64), ("zero_rest", c_int)]
 
 
 # name -> (restype, argtypes); every symbol declared in include/sesa.h
@@ -100,6 +130,11 @@ SIGNATURES = {
     "sesa_htdemucs_workspace_size": (c_size_t, [c_void_p, c_int]),
     "sesa_htdemucs_forward": (c_int, [c_void_p, P_f32, c_int, P_f32, c_void_p, c_size_t, c_void_p]),
     "sesa_htdemucs_destroy": (c_int, [c_void_p]),
+    "sesa_linear_i8": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_int64, c_int,
+                               c_int, c_void_p, c_int, c_int64, c_void_p]),
+    "sesa_norm_residual": (c_int, [ctypes.POINTER(SesaNormArgs), c_void_p]),
+    "sesa_rope_axes": (c_int, [ctypes.POINTER(SesaRopeArgs), c_void_p]),
+    "sesa_attention_packed": (c_int, [ctypes.POINTER(SesaAttnArgs), c_void_p]),
     "sesa_blend_workspace_size": (c_size_t, [c_int, c_int64]),
     "sesa_blend_workspace_size_n": (c_size_t, [c_int, c_int, c_int64]),
     "sesa_blend_f32": (c_int, [P_f32, c_int, c_int, c_int64, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_size_t,

@@ -238,3 +238,8 @@ def ola_counter(chunk, starts, seg_lens, window, counter):
 def ola_finalize(result, counter, border):
     """inference_pytorch.py:174-180 -> [n_out_ch, L_pad - 2*border]."""
     return torch.ops.sesa.ola_finalize(result, counter, int(border))
+
+
+# ---- transformer operators (sesa/token_ops.py) -----------------------------------------------------------
+from .token_ops import (attention_packed, linear_i8, norm_residual, norm_residual_i8, quantize_i8,  # noqa: E402,F401
+                        rope_axes, rope_axes_)
