@@ -51,7 +51,10 @@ __device__ __forceinline__ bool find_tile(const sesa_attn_args& a, int slot, int
   return q >= b && q < e;
 }
 
-template <class T, int D, int NW>
+// DMA: rows of exactly D elements at 16-byte addresses, K and V go to LDS by global_load_lds_dwordx4 (no registers, no
+// LDS stores; keys behind the sequence repeat its last one).  Otherwise through registers, zeros behind the sequence
+// and behind head_dim.
+template <class T, int D, int NW, bool DMA>
 __global__ void __launch_bounds__(NW * 64, 2) attn_packed_kernel(sesa_attn_args a, int n_slots) {
   constexpr int BQ = NW * 32, NTH = NW * 64, ROW = D * 2, IMG = kKeys * ROW, CH = D / 8, IT = kKeys * CH / NTH;
   constexpr float kLog2e = 1.4426950408889634f;
@@ -98,23 +101,48 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_packed_kernel(sesa_attn_args 
   const float c = a.scale * kLog2e;
 
   auto swz = [](int row, int chunk) { return row * ROW + ((chunk ^ (row & 7)) << 4); };
-  u32x4 kreg[IT], vreg[IT];
-  auto load_block = [&](int kb) {
+  // DMA piece i of this wave: LDS bytes 1024 (wave + NW i) .. of an image, lane * 16 into it; the swizzle goes on the
+  // source.  Offsets count from the block's first key.
+  constexpr int PCS = IMG / 1024 / NW, RPP = 1024 / ROW;   // pieces per wave and image, rows per piece
+  uint32_t koff[DMA ? PCS : 1], voff[DMA ? PCS : 1];
+  auto offsets = [&](int n) {   // n: keys of the block that exist
 #pragma unroll
-    for (int i = 0; i < IT; ++i) {
-      const int e = tid + i * NTH, key = e / CH, d = e % CH * 8;
-      const int64_t p = (int64_t)start + kb * kKeys + key;
-      const bool ok = p < end && d < hd;   // zeros behind the sequence and behind head_dim
-      kreg[i] = ok ? load16(kp + p * a.k_t + d) : u32x4{0u, 0u, 0u, 0u};
-      vreg[i] = ok ? load16(vp + p * a.v_t + d) : u32x4{0u, 0u, 0u, 0u};
+    for (int i = 0; i < PCS; ++i) {
+      const int row = (wave + NW * i) * RPP + lane / CH, ch = (lane % CH) ^ (row & 7), r = min(row, n - 1);
+      koff[i] = (uint32_t)(r * (int)a.k_t + ch * 8) * 2u;
+      voff[i] = (uint32_t)(r * (int)a.v_t + ch * 8) * 2u;
+    }
+  };
+  u32x4 kreg[DMA ? 1 : IT], vreg[DMA ? 1 : IT];
+  auto load_block = [&](int kb, char* stage) {
+    const int64_t p0 = (int64_t)start + kb * kKeys;
+    if constexpr (DMA) {
+      if (p0 + kKeys > end) offsets((int)(end - p0));
+      const char* kb0 = reinterpret_cast<const char*>(kp + p0 * a.k_t);
+      const char* vb0 = reinterpret_cast<const char*>(vp + p0 * a.v_t);
+#pragma unroll
+      for (int i = 0; i < PCS; ++i) dma16(kb0 + koff[i], stage + (wave + NW * i) * 1024);
+#pragma unroll
+      for (int i = 0; i < PCS; ++i) dma16(vb0 + voff[i], stage + IMG + (wave + NW * i) * 1024);
+    } else {
+#pragma unroll
+      for (int i = 0; i < IT; ++i) {
+        const int e = tid + i * NTH, d = e % CH * 8;
+        const int64_t p = p0 + e / CH;
+        const bool ok = p < end && d < hd;
+        kreg[i] = ok ? load16(kp + p * a.k_t + d) : u32x4{0u, 0u, 0u, 0u};
+        vreg[i] = ok ? load16(vp + p * a.v_t + d) : u32x4{0u, 0u, 0u, 0u};
+      }
     }
   };
   auto store_block = [&](char* stage) {
+    if constexpr (!DMA) {
 #pragma unroll
-    for (int i = 0; i < IT; ++i) {
-      const int e = tid + i * NTH, off = swz(e / CH, e % CH);
-      *reinterpret_cast<u32x4*>(stage + off) = kreg[i];
-      *reinterpret_cast<u32x4*>(stage + IMG + off) = vreg[i];
+      for (int i = 0; i < IT; ++i) {
+        const int e = tid + i * NTH, off = swz(e / CH, e % CH);
+        *reinterpret_cast<u32x4*>(stage + off) = kreg[i];
+        *reinterpret_cast<u32x4*>(stage + IMG + off) = vreg[i];
+      }
     }
   };
   // V^T fragment (d-block db, keys 16 ks ..): lane half hl gets the keys 4 hl .. + 3 and 8 + 4 hl .. + 3 of its step,
@@ -132,13 +160,18 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_packed_kernel(sesa_attn_args 
 
   const int last = a.causal ? min(end, q0 + BQ) : end;   // keys from here on reach no query of the tile
   const int n_blocks = (last - start + kKeys - 1) / kKeys;
-  load_block(0);
+  if constexpr (DMA) offsets(kKeys);
+  load_block(0, smem);
   store_block(smem);
-  if (n_blocks > 1) load_block(1);
-  sesa_sync();
   for (int kb = 0; kb < n_blocks; ++kb) {
     const char* K = smem + (kb & 1) * 2 * IMG;
     const char* V = K + IMG;
+    char* next = smem + ((kb + 1) & 1) * 2 * IMG;
+    // this wave's part of block kb has landed; behind the barrier everyone's has, and everyone is done with block
+    // kb - 1, whose place block kb + 1 takes
+    if constexpr (DMA) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    sesa_sync();
+    if (kb + 1 < n_blocks) load_block(kb + 1, next);
     f32x16 s[2];
 #pragma unroll
     for (int rb = 0; rb < 2; ++rb) {
@@ -150,15 +183,10 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_packed_kernel(sesa_attn_args 
         s[rb] = mfma16<T>(kf, qf[ks], s[rb]);
       }
     }
-    // block kb + 1 (loaded an iteration ago) into the other stage, whose last reads the barrier below has closed
-    if (kb + 1 < n_blocks) {
-      store_block(smem + ((kb + 1) & 1) * 2 * IMG);
-      if (kb + 2 < n_blocks) load_block(kb + 2);
-    }
     const int key0 = start + kb * kKeys;
-    const bool diagonal = a.causal && key0 + kKeys - 1 > q0 + wave * 32;
-    if (diagonal || key0 + kKeys > end) {
-      const int64_t lim = a.causal ? min((int64_t)end - 1, q_pos) : (int64_t)end - 1;   // last key this query sees
+    const bool masked = key0 + kKeys > end || (a.causal && key0 + kKeys - 1 > q0 + wave * 32);
+    const int64_t lim = a.causal ? min((int64_t)end - 1, q_pos) : (int64_t)end - 1;   // last key this query sees
+    if (masked) {
 #pragma unroll
       for (int rb = 0; rb < 2; ++rb)
 #pragma unroll
@@ -195,12 +223,12 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_packed_kernel(sesa_attn_args 
         sum += p;
       }
     l_run += sum + __shfl_xor(sum, 32);
-    // A diagonal block multiplies probabilities of 0 with keys behind the query: harmless for finite v, but 0 * inf is
-    // NaN, so look for non-finite v there (exponent all ones) and take that block element by element if there is one.
+    // A masked block multiplies probabilities of 0 with the keys its rows do not see: harmless for finite v, but 0 * inf
+    // is NaN, so look for non-finite v there (exponent all ones) and take that block element by element if there is one.
     uint32_t bad = 0;
     constexpr uint32_t kExp = std::is_same<T, f16>::value ? 0x7c007c00u : 0x7f807f80u;
     constexpr uint32_t kOne = std::is_same<T, f16>::value ? 0x04000400u : 0x00800080u;
-    if (diagonal) {
+    if (masked) {
       for (int e = lane; e < IMG / 16; e += 64) {
         const u32x4 w = *reinterpret_cast<const u32x4*>(V + e * 16);
 #pragma unroll
@@ -208,6 +236,8 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_packed_kernel(sesa_attn_args 
       }
     }
     if (__ballot((bad & 0x80008000u) != 0)) {
+      int hide = hl;   // (opaque: keeps this rare path's addresses out of the loop's registers)
+      asm volatile("" : "+v"(hide));
 #pragma unroll
       for (int rb = 0; rb < 2; ++rb)
 #pragma unroll 1
@@ -217,12 +247,12 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_packed_kernel(sesa_attn_args 
           for (int half = 0; half < 2; ++half) {
             const float p = __shfl(mine, l32 + 32 * half);
             const int key = rb * 32 + (r & 3) + 8 * (r >> 2) + 4 * half;
-            if (key0 + key > q_pos) continue;
+            if (key0 + key > lim) continue;
 #pragma unroll
             for (int db = 0; db < D / 32; ++db)
 #pragma unroll
               for (int q = 0; q < 16; ++q) {
-                const int d = db * 32 + 8 * (q >> 2) + 4 * hl + (q & 3);
+                const int d = db * 32 + 8 * (q >> 2) + 4 * hide + (q & 3);
                 o[db][q] = fmaf(p, (float)*reinterpret_cast<const T*>(V + swz(key, d >> 3) + ((d & 7) << 1)), o[db][q]);
               }
           }
@@ -238,7 +268,7 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_packed_kernel(sesa_attn_args 
         for (int db = 0; db < D / 32; ++db) o[db] = mfma16<T>(vt(V, ks, db), pf, o[db]);
       }
     }
-    sesa_sync();
+    if (kb + 1 < n_blocks) store_block(next);
   }
 
   if (!q_ok) return;
@@ -262,10 +292,20 @@ int launch_attn(const sesa_attn_args& a, hipStream_t st) {
   const int64_t n_slots = a.tokens / (NW * 32) + a.n_seq + 2;
   const int64_t blocks = n_slots * a.heads * a.lanes;
   SESA_REQUIRE(blocks < (1ll << 31), SESA_ERR_INVALID, "attention_packed: too many tokens x heads x lanes");
-  if (a.head_dim <= 64)
-    hipLaunchKernelGGL((attn_packed_kernel<T, 64, NW>), dim3((unsigned)blocks), dim3(NW * 64), 0, st, a, (int)n_slots);
-  else
-    hipLaunchKernelGGL((attn_packed_kernel<T, 128, NW>), dim3((unsigned)blocks), dim3(NW * 64), 0, st, a, (int)n_slots);
+  // 16-byte rows of a whole tile width, and a block's byte offsets in 32 bits
+  auto dma = [&](int D) {
+    const int64_t strides = a.k_t | a.k_l | a.k_h | a.v_t | a.v_l | a.v_h;
+    return a.head_dim == D && strides % 8 == 0 && ((uintptr_t)a.k | (uintptr_t)a.v) % 16 == 0 && a.k_t >= 0 &&
+           a.v_t >= 0 && a.k_t < (1 << 23) && a.v_t < (1 << 23);
+  };
+  const dim3 grid((unsigned)blocks), block(NW * 64);
+  if (a.head_dim <= 64) {
+    if (dma(64)) hipLaunchKernelGGL((attn_packed_kernel<T, 64, NW, true>), grid, block, 0, st, a, (int)n_slots);
+    else hipLaunchKernelGGL((attn_packed_kernel<T, 64, NW, false>), grid, block, 0, st, a, (int)n_slots);
+  } else {
+    if (dma(128)) hipLaunchKernelGGL((attn_packed_kernel<T, 128, NW, true>), grid, block, 0, st, a, (int)n_slots);
+    else hipLaunchKernelGGL((attn_packed_kernel<T, 128, NW, false>), grid, block, 0, st, a, (int)n_slots);
+  }
   SESA_CHECK_LAUNCH();
   return SESA_OK;
 }

@@ -8,7 +8,8 @@ and residual between two blocks; rows in 8 bits), ``rope_axes`` / ``rope_axes_``
 Device tensors only, on the current stream of the tensors' device; every result is a new tensor unless the name says
 otherwise; nothing waits for the device, so the calls can be captured into a graph.  Inference only: a call whose
 inputs would need a gradient raises.  The ops are plain ``torch.library`` definitions (schema, device kernel, fake
-kernel): for a single token the host's share of a call is most of it, and this form has the least.
+kernel), and an eager call of the functions below goes straight to the device kernel: for a single token the host's
+share of a call is most of it.
 """
 import ctypes
 
@@ -40,34 +41,49 @@ def _fail(op, msg):
     raise N.SesaError(f"sesa::{op}: {msg}")
 
 
-def _check(op, dev, **tensors):
-    """Every tensor (None: absent) on ``dev``, none of them waiting for a gradient."""
-    for name, t in tensors.items():
+def _check(op, idx, names, *tensors):
+    """Every tensor (None: absent) on device ``idx``, none of them waiting for a gradient."""
+    grad = torch.is_grad_enabled()
+    for i, t in enumerate(tensors):
         if t is None:
             continue
-        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.device != dev:
-            _fail(op, f"{name}: expected a HIP device tensor on {dev} (got {type(t).__name__} on "
+        if not isinstance(t, torch.Tensor) or t.get_device() != idx:
+            _fail(op, f"{names.split()[i]}: expected a HIP device tensor on cuda:{idx} (got {type(t).__name__} on "
                       f"{getattr(t, 'device', None)}); the sesa path has no CPU fallback")
-        if t.requires_grad and torch.is_grad_enabled():
-            _fail(op, f"{name} requires a gradient and this operator has none (use torch.no_grad())")
+        if grad and t.requires_grad:
+            _fail(op, f"{names.split()[i]} requires a gradient and this operator has none (use torch.no_grad())")
 
 
 def _device(op, t):
+    """The index of the device the call runs on."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         _fail(op, f"expected a HIP device tensor (got {type(t).__name__} on {getattr(t, 'device', None)}); "
                   "the sesa path has no CPU fallback")
-    return t.device
+    return t.get_device()
 
 
-def _launch(op, dev, call):
-    """``call(stream)`` with ``dev`` current, on its current stream."""
-    if torch.cuda.current_device() == dev.index:
-        rc = call(torch.cuda.current_stream(dev).cuda_stream)
+def _launch(op, idx, entry, *args):
+    """``entry(*args, stream)`` with device ``idx`` current, on its current stream."""
+    if torch.cuda.current_device() == idx:
+        rc = entry(*args, torch._C._cuda_getCurrentRawStream(idx))
     else:
-        with torch.cuda.device(dev):
-            rc = call(torch.cuda.current_stream(dev).cuda_stream)
+        with torch.cuda.device(idx):
+            rc = entry(*args, torch._C._cuda_getCurrentRawStream(idx))
     if rc:
         N.check(rc, f"sesa_{op}")
+
+
+_modes = getattr(torch._C, "_len_torch_dispatch_stack", lambda: 1)
+
+
+def _eager(op, t):
+    """Whether a call can go straight to its device kernel: a plain device tensor, nothing tracing or intercepting the
+    ops.  Saves the dispatcher's share of the host's time (3 to 4 us a call: a one-token call takes 5 to 8)."""
+    if type(t) is torch.Tensor:
+        _device(op, t)
+        return not torch.compiler.is_compiling() and not _modes()
+    _device(op, t)
+    return False
 
 
 def _param(op, name, t, n):
@@ -83,7 +99,7 @@ def _rows(t):
     """[..., n] as [rows, n] with the last dimension contiguous (a copy only where the strides need one)."""
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1])
-    return t if t.shape[1] <= 1 or t.stride(1) == 1 else t.contiguous()
+    return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
 
 
 def _span(t):
@@ -132,8 +148,8 @@ def _linear_shape(x, x_scale, weight):
          "ScalarType out_dtype) -> Tensor")
 def _linear_i8(x, x_scale, weight, w_scale, bias, act, out_dtype):
     op = "linear_i8"
-    dev = _device(op, x)
-    _check(op, dev, x_scale=x_scale, weight=weight, w_scale=w_scale, bias=bias)
+    idx = _device(op, x)
+    _check(op, idx, "x x_scale weight w_scale bias", x, x_scale, weight, w_scale, bias)
     shape = _linear_shape(x, x_scale, weight)
     if x.dtype != torch.int8 or weight.dtype != torch.int8:
         _fail(op, f"x and weight: expected int8, got {x.dtype} and {weight.dtype}")
@@ -145,10 +161,9 @@ def _linear_i8(x, x_scale, weight, w_scale, bias, act, out_dtype):
     ws, b = _param(op, "w_scale", w_scale, n), _param(op, "bias", bias, n)
     xr, wr = _rows(x), _rows(weight)
     xs = x_scale if x_scale.is_contiguous() else x_scale.contiguous()
-    out = torch.empty(shape, device=dev, dtype=out_dtype)
-    _launch(op, dev, lambda st: N.lib().sesa_linear_i8(
-        xr.data_ptr(), xr.stride(0), xs.data_ptr(), wr.data_ptr(), wr.stride(0), ws.data_ptr(), _ptr(b), _ACT[act],
-        xr.shape[0], n, k, out.data_ptr(), _DTYPE[out_dtype], n, st))
+    out = x.new_empty(shape, dtype=out_dtype)
+    _launch(op, idx, N.lib().sesa_linear_i8, xr.data_ptr(), xr.stride(0), xs.data_ptr(), wr.data_ptr(), wr.stride(0),
+            ws.data_ptr(), _ptr(b), _ACT[act], xr.shape[0], n, k, out.data_ptr(), _DTYPE[out_dtype], n)
     return out
 
 
@@ -178,9 +193,9 @@ def _gate_groups(x, gate):
 
 
 def _norm_call(op, x, residual, gate, gate_act, post, post_weight, post_bias, scale, pre, pre_weight, pre_bias, eps, i8):
-    dev = _device(op, x)
-    _check(op, dev, x=x, residual=residual, gate=gate, post_weight=post_weight, post_bias=post_bias, scale=scale,
-           pre_weight=pre_weight, pre_bias=pre_bias)
+    idx = _device(op, x)
+    _check(op, idx, "x residual gate post_weight post_bias scale pre_weight pre_bias", x, residual, gate, post_weight,
+           post_bias, scale, pre_weight, pre_bias)
     if x.dtype not in _DTYPE or x.dim() < 1:
         _fail(op, f"x: expected float32, float16 or bfloat16 [..., dim], got {x.dtype} {list(x.shape)}")
     if post not in _NORM or pre not in _NORM or gate_act not in _GATE:
@@ -195,19 +210,19 @@ def _norm_call(op, x, residual, gate, gate_act, post, post_weight, post_bias, sc
     per = 1 if gate is None else _gate_groups(x, gate)
     rt = x.dtype if residual is None else residual.dtype
     xr = _rows(x)
-    rr, gr = (None if t is None else _rows(t) for t in (residual, gate))
-    y = torch.empty(x.shape, device=dev, dtype=rt)
-    n = torch.empty(x.shape, device=dev, dtype=torch.int8 if i8 else x.dtype)
-    qs = torch.empty(x.shape[:-1], device=dev, dtype=torch.float32) if i8 else None
-    pw, pb, sc = (_param(op, a, t, d) for a, t in (("post_weight", post_weight), ("post_bias", post_bias),
-                                                   ("scale", scale)))
+    rr, gr = None if residual is None else _rows(residual), None if gate is None else _rows(gate)
+    y = x.new_empty(x.shape, dtype=rt)
+    n = x.new_empty(x.shape, dtype=torch.int8) if i8 else x.new_empty(x.shape)
+    qs = x.new_empty(x.shape[:-1], dtype=torch.float32) if i8 else None
+    pw, pb = _param(op, "post_weight", post_weight, d), _param(op, "post_bias", post_bias, d)
     nw, nb = _param(op, "pre_weight", pre_weight, d), _param(op, "pre_bias", pre_bias, d)
+    sc = _param(op, "scale", scale, d)
     a = N.SesaNormArgs(
         xr.shape[0], d, _DTYPE[x.dtype], _DTYPE[rt], xr.data_ptr(), xr.stride(0), _ptr(rr),
         0 if rr is None else rr.stride(0), _ptr(gr), 0 if gr is None else gr.stride(0), per, _GATE[gate_act],
         _NORM[post], _ptr(pw), _ptr(pb), _ptr(sc), _NORM[pre], _ptr(nw), _ptr(nb), eps, y.data_ptr(), d,
         None if i8 else n.data_ptr(), d, n.data_ptr() if i8 else None, d, _ptr(qs))
-    _launch("norm_residual", dev, lambda st: N.lib().sesa_norm_residual(ctypes.byref(a), st))
+    _launch("norm_residual", idx, N.lib().sesa_norm_residual, ctypes.byref(a))
     return (y, n, qs) if i8 else (y, n)
 
 
@@ -241,16 +256,16 @@ def _(x, residual, *rest):
 @_define("quantize_i8(Tensor x) -> (Tensor, Tensor)")
 def _quantize_i8(x):
     op = "quantize_i8"
-    dev = _device(op, x)
-    _check(op, dev, x=x)
+    idx = _device(op, x)
+    _check(op, idx, "x", x)
     if x.dtype not in _DTYPE or x.dim() < 1:
         _fail(op, f"x: expected float32, float16 or bfloat16 [..., dim], got {x.dtype} {list(x.shape)}")
     xr = _rows(x)
-    q = torch.empty(x.shape, device=dev, dtype=torch.int8)
-    s = torch.empty(x.shape[:-1], device=dev, dtype=torch.float32)
+    q = x.new_empty(x.shape, dtype=torch.int8)
+    s = x.new_empty(x.shape[:-1], dtype=torch.float32)
     a = N.SesaNormArgs(rows=xr.shape[0], dim=x.shape[-1], x_dtype=_DTYPE[x.dtype], r_dtype=_DTYPE[x.dtype],
                        x=xr.data_ptr(), x_ld=xr.stride(0), q=q.data_ptr(), q_ld=x.shape[-1], q_scale=s.data_ptr())
-    _launch("norm_residual", dev, lambda st: N.lib().sesa_norm_residual(ctypes.byref(a), st))
+    _launch("norm_residual", idx, N.lib().sesa_norm_residual, ctypes.byref(a))
     return q, s
 
 
@@ -262,8 +277,8 @@ def _(x):
 
 # ---- rope_axes ------------------------------------------------------------------------------------------
 def _rope_call(op, xs, outs, positions, freqs, sections, layout):
-    dev = _device(op, xs[0])
-    _check(op, dev, positions=positions, freqs=freqs, **{f"tensor {i}": x for i, x in enumerate(xs)})
+    idx = _device(op, xs[0])
+    _check(op, idx, "positions freqs q k", positions, freqs, *xs)
     x0 = xs[0]
     for x in xs:
         if x.dim() != 3 or x.dtype not in _DTYPE or x.dtype != x0.dtype or x.shape[0] != x0.shape[0] or \
@@ -285,7 +300,7 @@ def _rope_call(op, xs, outs, positions, freqs, sections, layout):
     for i, (x, o) in enumerate(zip(xs, outs)):
         a.t[i] = N.SesaRopeTensor(x.data_ptr(), x.stride(0), x.stride(1), o.data_ptr(), o.stride(0), o.stride(1),
                                   x.shape[1])
-    _launch("rope_axes", dev, lambda st: N.lib().sesa_rope_axes(ctypes.byref(a), st))
+    _launch("rope_axes", idx, N.lib().sesa_rope_axes, ctypes.byref(a))
 
 
 @_define("rope_axes(Tensor[] xs, Tensor positions, Tensor freqs, int[] sections, str layout) -> Tensor[]")
@@ -294,7 +309,7 @@ def _rope_axes(xs, positions, freqs, sections, layout):
         _fail("rope_axes", f"one or two tensors, got {len(xs)}")
     _device("rope_axes", xs[0])
     xs = [x if x.dim() < 1 or x.stride(-1) == 1 else x.contiguous() for x in xs]
-    outs = [torch.empty(x.shape, device=x.device, dtype=x.dtype) for x in xs]
+    outs = [x.new_empty(x.shape) for x in xs]
     _rope_call("rope_axes", xs, outs, positions, freqs, sections, layout)
     return outs
 
@@ -325,8 +340,8 @@ def _(xs, positions, freqs, sections, layout):
 
 # ---- attention_packed -----------------------------------------------------------------------------------
 def _attn_call(op, q, k, v, cu, causal, scale, gate, out, zero_rest):
-    dev = _device(op, q)
-    _check(op, dev, q=q, k=k, v=v, cu_seqlens=cu, gate=gate, out=out)
+    idx = _device(op, q)
+    _check(op, idx, "q k v cu_seqlens gate out", q, k, v, cu, gate, out)
     if q.dtype not in (torch.float16, torch.bfloat16) or k.dtype != q.dtype or v.dtype != q.dtype:
         _fail(op, f"q, k, v: expected one of float16 and bfloat16, got {q.dtype}, {k.dtype}, {v.dtype}")
     nd = q.dim()
@@ -354,13 +369,14 @@ def _attn_call(op, q, k, v, cu, causal, scale, gate, out, zero_rest):
                        1 if cu is None else cu.shape[0] - 1, causal,
                        q.shape[-1] ** -0.5 if scale is None else scale, _ptr(gate),
                        *((0, 0, 0) if gate is None else st3(gate, 0)), out.data_ptr(), *st3(out, 1), zero_rest)
-    _launch("attention_packed", dev, lambda st: N.lib().sesa_attention_packed(ctypes.byref(a), st))
+    _launch("attention_packed", idx, N.lib().sesa_attention_packed, ctypes.byref(a))
 
 
 @_define("attention_packed(Tensor q, Tensor k, Tensor v, Tensor? cu_seqlens, bool causal, float? scale, Tensor? gate) "
          "-> Tensor")
 def _attention_packed(q, k, v, cu_seqlens, causal, scale, gate):
-    out = torch.empty(q.shape, device=_device("attention_packed", q), dtype=q.dtype)
+    _device("attention_packed", q)
+    out = q.new_empty(q.shape)
     _attn_call("attention_packed", q, k, v, cu_seqlens, causal, scale, gate, out, True)
     return out
 
@@ -391,18 +407,14 @@ def _(q, k, v, cu_seqlens, causal, scale, gate, out):
 
 
 # ---- Python entry points --------------------------------------------------------------------------------
-def _dev(op, t):
-    _device(op, t)
-    return t
-
-
 def linear_i8(x, x_scale, weight, w_scale, bias=None, *, act="none", out_dtype=torch.float16):
     """``act(x_scale * w_scale * (x @ weight.T) + bias)`` on 8-bit integers -> [..., n] in ``out_dtype``.
 
     x int8 [..., k] with x_scale fp32 [...] (one scale a token), weight int8 [n, k] with w_scale fp32 [n] (one a channel;
     ``quantize_i8`` makes both pairs), bias fp32 [n] or None; act 'none', 'gelu' (erf), 'tanh' or 'relu'.  The sum is an
     exact 32-bit integer (k <= 131071), everything after it fp32, rounded once."""
-    return torch.ops.sesa.linear_i8(_dev("linear_i8", x), x_scale, weight, w_scale, bias, act, out_dtype)
+    call = _linear_i8 if _eager("linear_i8", x) else torch.ops.sesa.linear_i8
+    return call(x, x_scale, weight, w_scale, bias, act, out_dtype)
 
 
 def norm_residual(x, residual=None, *, gate=None, gate_act="none", post="none", post_weight=None, post_bias=None,
@@ -414,8 +426,8 @@ def norm_residual(x, residual=None, *, gate=None, gate_act="none", post="none", 
     gate that many rows share ([groups, dim] for x [rows, dim]); gate_act 'none', 'sigmoid', 'silu' or 'tanh'.
     post / pre: 'none', 'rms' or 'layer' with fp32 [dim] weights (None: 1) and biases (None: 0); scale fp32 [dim].
     Statistics are fp32; y and n are rounded once, n from the unrounded y."""
-    return torch.ops.sesa.norm_residual(_dev("norm_residual", x), residual, gate, gate_act, post, post_weight, post_bias,
-                                        scale, pre, pre_weight, pre_bias, eps)
+    call = _norm_residual if _eager("norm_residual", x) else torch.ops.sesa.norm_residual
+    return call(x, residual, gate, gate_act, post, post_weight, post_bias, scale, pre, pre_weight, pre_bias, eps)
 
 
 def norm_residual_i8(x, residual=None, *, gate=None, gate_act="none", post="none", post_weight=None, post_bias=None,
@@ -424,13 +436,13 @@ def norm_residual_i8(x, residual=None, *, gate=None, gate_act="none", post="none
 
     q_scale = max |n| / 127, q = round(n / q_scale) to even.  An all-zero row has scale 0; a row that holds a NaN or an
     infinity has scale NaN and q 0, so a product with it is NaN in every channel."""
-    return torch.ops.sesa.norm_residual_i8(_dev("norm_residual_i8", x), residual, gate, gate_act, post, post_weight,
-                                           post_bias, scale, pre, pre_weight, pre_bias, eps)
+    call = _norm_residual_i8 if _eager("norm_residual_i8", x) else torch.ops.sesa.norm_residual_i8
+    return call(x, residual, gate, gate_act, post, post_weight, post_bias, scale, pre, pre_weight, pre_bias, eps)
 
 
 def quantize_i8(x):
     """Rows in 8 bits, one scale a row (``norm_residual_i8``'s rule, no norm): weights [n, k], activations [..., k]."""
-    return torch.ops.sesa.quantize_i8(_dev("quantize_i8", x))
+    return (_quantize_i8 if _eager("quantize_i8", x) else torch.ops.sesa.quantize_i8)(x)
 
 
 def rope_axes(q, k, positions, freqs, sections, *, layout="halves"):
@@ -439,15 +451,15 @@ def rope_axes(q, k, positions, freqs, sections, *, layout="halves"):
     positions int32 / int64 [tokens, axes] (any value; angles are reduced exactly), sections the number of pairs each axis
     turns, freqs fp32 [sum(sections)] in radians per position.  layout 'halves': pair i = elements (i, i + P), P =
     sum(sections); 'pairs': (2 i, 2 i + 1).  Elements behind the pairs pass through."""
-    xs = [_dev("rope_axes", q)] if k is None else [_dev("rope_axes", q), k]
-    out = torch.ops.sesa.rope_axes(xs, positions, freqs, sections, layout)
+    call = _rope_axes if _eager("rope_axes", q) else torch.ops.sesa.rope_axes
+    out = call([q] if k is None else [q, k], positions, freqs, sections, layout)
     return out[0] if k is None else (out[0], out[1])
 
 
 def rope_axes_(q, k, positions, freqs, sections, *, layout="halves"):
     """``rope_axes`` in place on q and k (k may be None)."""
-    torch.ops.sesa.rope_axes_([_dev("rope_axes_", q)] if k is None else [_dev("rope_axes_", q), k], positions, freqs,
-                              sections, layout)
+    _device("rope_axes_", q)
+    torch.ops.sesa.rope_axes_([q] if k is None else [q, k], positions, freqs, sections, layout)
 
 
 def attention_packed(q, k, v, cu_seqlens=None, *, causal=True, scale=None, gate=None, out=None):
@@ -459,8 +471,9 @@ def attention_packed(q, k, v, cu_seqlens=None, *, causal=True, scale=None, gate=
     cu_seqlens int32 [sequences + 1] on the device: sequence s is tokens cu_seqlens[s] .. cu_seqlens[s + 1] - 1 (None:
     one sequence).  gate: logits [tokens, (lanes,) heads], a sigmoid on each head's output.  scale: head_dim ** -0.5.
     Rows of no sequence (behind the last) come back 0; with ``out`` they are left as they were."""
-    _dev("attention_packed", q)
+    eager = _eager("attention_packed", q)
     if out is None:
-        return torch.ops.sesa.attention_packed(q, k, v, cu_seqlens, causal, scale, gate)
+        call = _attention_packed if eager else torch.ops.sesa.attention_packed
+        return call(q, k, v, cu_seqlens, causal, scale, gate)
     torch.ops.sesa.attention_packed_into(q, k, v, cu_seqlens, causal, scale, gate, out)
     return out
