@@ -100,7 +100,12 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_packed_kernel(sesa_attn_args 
   float m_run = -INFINITY, l_run = 0.f;   // running maximum (of the raw scores) and sum
   const float c = a.scale * kLog2e;
 
-  auto swz = [](int row, int chunk) { return row * ROW + ((chunk ^ (row & 7)) << 4); };
+  // 16-byte chunk c of row r lies at c ^ key(r).  A K fragment read takes one chunk of 8 rows at a time, a transposing V
+  // read four chunks of 4 rows: both sets fall into different banks (256 B of them: two rows of 64 elements, one of 128).
+  auto key_of = [](int row) {
+    return D == 64 ? ((row << 1) & 4) | ((row >> 2) & 3) : ((row & 3) << 2) | ((row >> 2) & 3);
+  };
+  auto swz = [&](int row, int chunk) { return row * ROW + ((chunk ^ key_of(row)) << 4); };
   // DMA piece i of this wave: LDS bytes 1024 (wave + NW i) .. of an image, lane * 16 into it; the swizzle goes on the
   // source.  Offsets count from the block's first key.
   constexpr int PCS = IMG / 1024 / NW, RPP = 1024 / ROW;   // pieces per wave and image, rows per piece
@@ -108,7 +113,7 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_packed_kernel(sesa_attn_args 
   auto offsets = [&](int n) {   // n: keys of the block that exist
 #pragma unroll
     for (int i = 0; i < PCS; ++i) {
-      const int row = (wave + NW * i) * RPP + lane / CH, ch = (lane % CH) ^ (row & 7), r = min(row, n - 1);
+      const int row = (wave + NW * i) * RPP + lane / CH, ch = (lane % CH) ^ key_of(row), r = min(row, n - 1);
       koff[i] = (uint32_t)(r * (int)a.k_t + ch * 8) * 2u;
       voff[i] = (uint32_t)(r * (int)a.v_t + ch * 8) * 2u;
     }

@@ -30,11 +30,22 @@ __device__ __forceinline__ i32x4 mfma_i8(i32x4 a, i32x4 b, i32x4 c) {
   return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
 }
 
-__device__ __forceinline__ float activate(float v, int act) {
-  if (act == SESA_ACT_GELU) return gelu_erf(v);
-  if (act == SESA_ACT_TANH) return tanh_f(v);
-  if (act == SESA_ACT_RELU) return v > 0.f || v != v ? v : 0.f;   // (keeps NaN)
+template <int ACT>
+__device__ __forceinline__ float activate(float v) {
+  if constexpr (ACT == SESA_ACT_GELU) return gelu_erf(v);
+  if constexpr (ACT == SESA_ACT_TANH) return tanh_f(v);
+  if constexpr (ACT == SESA_ACT_RELU) return v > 0.f || v != v ? v : 0.f;   // (keeps NaN)
   return v;
+}
+
+// body(activation as a constant): one copy of an epilogue per activation and one branch around them, where a branch per
+// element made the epilogue 12000 instructions and slower than the product (m 49662, k 512, n 2048: 130 us of 164)
+template <class F>
+__device__ __forceinline__ void with_act(int act, F body) {
+  if (act == SESA_ACT_NONE) body(std::integral_constant<int, SESA_ACT_NONE>{});
+  else if (act == SESA_ACT_GELU) body(std::integral_constant<int, SESA_ACT_GELU>{});
+  else if (act == SESA_ACT_TANH) body(std::integral_constant<int, SESA_ACT_TANH>{});
+  else body(std::integral_constant<int, SESA_ACT_RELU>{});
 }
 
 // 16 bytes of a row from byte k on, zero from byte K on
@@ -48,13 +59,13 @@ __device__ __forceinline__ i32x4 load_k(const int8_t* row, int k, int K) {
 }
 
 // ---------------------------------------------------------------------------------------------
-constexpr int kBK = 128;   // K bytes per stage: one row is 8 16-byte pieces
-
-// LDS image of a stage: rows of 128 B, piece c of row r at position c ^ key(r), so that the 8 rows whose pieces a
-// fragment read takes together lie in 8 different piece columns.  Token fragments take 16 consecutive rows; weight
-// fragments rows {0..3, 16..19, 32..35, 48..51} + 4 j of a 64-row group (see tile_kernel).
-__device__ __forceinline__ int key_x(int r) { return r & 7; }
-__device__ __forceinline__ int key_w(int r) { return (r & 3) | ((r >> 2) & 4); }
+// LDS image of a stage: rows of BK bytes, 16-byte piece c of row r at position c ^ key(r), so that the 8 rows whose pieces
+// a fragment read takes together lie in 8 different 16-byte columns of 128 B.  Token fragments take 16 consecutive rows;
+// weight fragments rows {0..3, 16..19, 32..35, 48..51} + 4 j of a 64-row group (see tile_kernel).
+template <int BK>
+__device__ __forceinline__ int key_x(int r) { return BK == 128 ? r & 7 : (r >> 1) & 3; }
+template <int BK>
+__device__ __forceinline__ int key_w(int r) { return BK == 128 ? (r & 3) | ((r >> 2) & 4) : ((r >> 1) & 1) | ((r >> 3) & 2); }
 
 // WAN x WAM waves, each GN groups of 64 channels x GM blocks of 16 tokens.
 // Channel order: accumulator block j (0..3) of a 64-channel group holds, in row 4 g + i of the matrix instruction,
@@ -62,39 +73,43 @@ __device__ __forceinline__ int key_w(int r) { return (r & 3) | ((r >> 2) & 4); }
 // group) and the epilogue stores straight from registers.
 // DMA: rows 16-byte aligned and K % 16 == 0 -- stages filled by global_load_lds_dwordx4 (the swizzle on the source
 // address).  Otherwise through registers, where the last partial piece of a row is completed with zeros.
-template <class TO, int WAN, int WAM, int GN, int GM, bool DMA>
-__global__ void __launch_bounds__(WAN* WAM * 64, 2) tile_kernel(LinArgs a) {
+template <class TO, int WAN, int WAM, int GN, int GM, int BK, int OCC, bool DMA>
+__global__ void __launch_bounds__(WAN* WAM * 64, OCC) tile_kernel(LinArgs a) {
   constexpr int NW = WAN * WAM, BN = WAN * GN * 64, BM = WAM * GM * 16;
-  constexpr int STAGE = (BN + BM) * kBK, PIECES = STAGE / 1024 / NW, WP = BN * kBK / 1024 / NW;   // per wave
-  static_assert(STAGE % (1024 * NW) == 0 && BN * kBK % (1024 * NW) == 0, "whole pieces per wave");
+  constexpr int STAGE = (BN + BM) * BK, PIECES = STAGE / 1024 / NW, WP = BN * BK / 1024 / NW;   // per wave
+  constexpr int LPR = BK / 16, RPP = 64 / LPR;   // lanes per row, rows per piece
+  static_assert(STAGE % (1024 * NW) == 0 && BN * BK % (1024 * NW) == 0, "whole pieces per wave");
   __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];
+  float* xs_l = reinterpret_cast<float*>(smem);   // the tile's scales and bias, once the stages are done
+  float* ws_l = xs_l + BM;
+  float* b_l = ws_l + BN;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int wn = wave % WAN, wm = wave / WAN;
   const int tiles_n = (a.n + BN - 1) / BN, tiles_m = (a.m + BM - 1) / BM;
-  // within a die's range: strips of 4 token tiles, channels along the strip
+  const int steps = (a.k + BK - 1) / BK;
+  // within a die's range of tiles: strips of 4 token tiles, channels along the strip
   const int t = die_tile(blockIdx.x, gridDim.x);
   constexpr int STRIP = 4;
   const int strip = t / (STRIP * tiles_n), in = t - strip * STRIP * tiles_n;
   const int sm = min(STRIP, tiles_m - strip * STRIP);
   const int m0 = (strip * STRIP + in % sm) * BM, n0 = in / sm * BN;
-  const int steps = (a.k + kBK - 1) / kBK;
 
-  // piece p of this wave: rows 8 (wave + NW p) .. + 7 of the weight (p < WP) or token image, 8 lanes a row
+  // piece p of this wave: RPP rows from RPP (wave + NW p) on of the weight (p < WP) or token image
   const int8_t* src[PIECES];
   int piece[PIECES];
 #pragma unroll
   for (int p = 0; p < PIECES; ++p) {
     const bool is_w = p < WP;
-    const int r = 8 * (wave + NW * (is_w ? p : p - WP)) + (lane >> 3);
-    piece[p] = 16 * ((lane & 7) ^ (is_w ? key_w(r) : key_x(r)));
+    const int r = RPP * (wave + NW * (is_w ? p : p - WP)) + lane / LPR;
+    piece[p] = 16 * (lane % LPR ^ (is_w ? key_w<BK>(r) : key_x<BK>(r)));
     src[p] = is_w ? a.w + (int64_t)min(n0 + r, a.n - 1) * a.w_ld : a.x + (int64_t)min(m0 + r, a.m - 1) * a.x_ld;
   }
   u32x4 held[DMA ? 1 : PIECES];
-  auto lds_at = [&](int p) { return (p < WP ? 0 : BN * kBK) + (wave + NW * (p < WP ? p : p - WP)) * 1024; };
+  auto lds_at = [&](int p) { return (p < WP ? 0 : BN * BK) + (wave + NW * (p < WP ? p : p - WP)) * 1024; };
   auto fetch = [&](int s, char* stage) {
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
-      const int k = s * kBK + piece[p];
+      const int k = s * BK + piece[p];
       if constexpr (DMA) {   // pieces past K: any valid address (their products are masked in the last step)
         dma16(src[p] + (k < a.k ? k : 0), stage + lds_at(p));
       } else {
@@ -110,31 +125,24 @@ __global__ void __launch_bounds__(WAN* WAM * 64, 2) tile_kernel(LinArgs a) {
   };
 
   i32x4 acc[GN][4][GM];
-#pragma unroll
-  for (int u = 0; u < GN; ++u)
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int i = 0; i < GM; ++i) acc[u][j][i] = i32x4{0, 0, 0, 0};
-
   const int l16 = lane & 15, g = lane >> 4;
   auto compute = [&](const char* stage, int s) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int k0 = s * kBK + h * 64;
+    for (int h = 0; h < BK / 64; ++h) {
+      const int k0 = s * BK + h * 64;
       if (k0 >= a.k) break;
       i32x4 wf[GN][4], xf[GM];
 #pragma unroll
       for (int i = 0; i < GM; ++i) {
         const int r = (wm * GM + i) * 16 + l16;
-        xf[i] = *reinterpret_cast<const i32x4*>(stage + BN * kBK + r * kBK + 16 * ((h * 4 + g) ^ key_x(r)));
+        xf[i] = *reinterpret_cast<const i32x4*>(stage + BN * BK + r * BK + 16 * ((h * 4 + g) ^ key_x<BK>(r)));
       }
 #pragma unroll
       for (int u = 0; u < GN; ++u)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int r = (wn * GN + u) * 64 + (l16 >> 2) * 16 + j * 4 + (l16 & 3);
-          wf[u][j] = *reinterpret_cast<const i32x4*>(stage + r * kBK + 16 * ((h * 4 + g) ^ key_w(r)));
+          wf[u][j] = *reinterpret_cast<const i32x4*>(stage + r * BK + 16 * ((h * 4 + g) ^ key_w<BK>(r)));
         }
       if (DMA && k0 + 64 > a.k && k0 + 16 * g >= a.k) {   // (K % 16 == 0: whole pieces lie inside or outside)
 #pragma unroll
@@ -149,13 +157,19 @@ __global__ void __launch_bounds__(WAN* WAM * 64, 2) tile_kernel(LinArgs a) {
     }
   };
 
+#pragma unroll
+  for (int u = 0; u < GN; ++u)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < GM; ++i) acc[u][j][i] = i32x4{0, 0, 0, 0};
   fetch(0, smem);
   put(smem);
   for (int s = 0; s < steps; ++s) {
     char* cur = smem + (s & 1) * STAGE;
     char* next = smem + ((s + 1) & 1) * STAGE;
-    // this wave's part of stage s has landed; after the barrier everyone's has, and everyone is done reading stage
-    // s - 1, whose place stage s + 1 takes
+    // this wave's part of stage s has landed; behind the barrier everyone's has, and everyone is done with stage s - 1,
+    // whose place stage s + 1 takes
     if constexpr (DMA) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     sesa_sync();
     if (s + 1 < steps) fetch(s + 1, next);
@@ -163,47 +177,41 @@ __global__ void __launch_bounds__(WAN* WAM * 64, 2) tile_kernel(LinArgs a) {
     if (s + 1 < steps) put(next);
   }
 
-  TO* out = reinterpret_cast<TO*>(a.out);
-#pragma unroll
-  for (int u = 0; u < GN; ++u) {
-    const int n = n0 + (wn * GN + u) * 64 + 16 * g, left = a.n - n;
-    float ws[16], b[16];
-    {
-      float lo[8], hi[8];
-      load8(a.w_scale + n, left, lo);
-      load8(a.w_scale + n + 8, left - 8, hi);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) { ws[e] = lo[e]; ws[8 + e] = hi[e]; }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) lo[e] = hi[e] = 0.f;
-      if (a.bias) {
-        load8(a.bias + n, left, lo);
-        load8(a.bias + n + 8, left - 8, hi);
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) { b[e] = lo[e]; b[8 + e] = hi[e]; }
-    }
-#pragma unroll
-    for (int i = 0; i < GM; ++i) {
-      const int m = m0 + (wm * GM + i) * 16 + l16;
-      const float xs = a.x_scale[min(m, a.m - 1)];
-      float lo[8], hi[8];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int c = 4 * j + e;
-          const float v = activate(fmaf((float)acc[u][j][i][e], xs * ws[c], b[c]), a.act);
-          if (c < 8) lo[c] = v;
-          else hi[c - 8] = v;
-        }
-      if (m < a.m && left > 0) {
-        TO* o = out + (int64_t)m * a.o_ld + n;
-        store8(o, left, lo);
-        store8(o + 8, left - 8, hi);
-      }
-    }
+  sesa_sync();
+  for (int e = tid; e < BM; e += NW * 64) xs_l[e] = a.x_scale[min(m0 + e, a.m - 1)];
+  for (int e = tid; e < BN; e += NW * 64) {
+    const int n = min(n0 + e, a.n - 1);
+    ws_l[e] = a.w_scale[n];
+    b_l[e] = a.bias ? a.bias[n] : 0.f;
   }
+  sesa_sync();
+  TO* out = reinterpret_cast<TO*>(a.out);
+  with_act(a.act, [&](auto act) {
+    constexpr int ACT = decltype(act)::value;
+#pragma unroll
+    for (int u = 0; u < GN; ++u) {
+      const int c0 = (wn * GN + u) * 64 + 16 * g, n = n0 + c0, left = a.n - n;
+#pragma unroll
+      for (int i = 0; i < GM; ++i) {
+        const int r = (wm * GM + i) * 16 + l16, m = m0 + r;
+        const float xs = xs_l[r];
+        float v[2][8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const f32x4 w4 = *reinterpret_cast<const f32x4*>(ws_l + c0 + 4 * j);
+          const f32x4 b4 = *reinterpret_cast<const f32x4*>(b_l + c0 + 4 * j);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            v[j >> 1][4 * (j & 1) + e] = activate<ACT>(fmaf((float)acc[u][j][i][e], xs * w4[e], b4[e]));
+        }
+        if (m < a.m && left > 0) {
+          TO* o = out + (int64_t)m * a.o_ld + n;
+          store8(o, left, v[0]);
+          store8(o + 8, left - 8, v[1]);
+        }
+      }
+    }
+  });
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -247,27 +255,29 @@ __global__ void __launch_bounds__(256) few_kernel(LinArgs a) {
   for (int i = 0; i < MI; ++i) part[wave][i][lane] = acc[i];
   sesa_sync();
   TO* out = reinterpret_cast<TO*>(a.out);
-  for (int i = wave; i < MI; i += NW) {
-    i32x4 v = part[0][i][lane];
+  with_act(a.act, [&](auto act) {
+    for (int i = wave; i < MI; i += NW) {
+      i32x4 v = part[0][i][lane];
 #pragma unroll
-    for (int w = 1; w < NW; ++w) v += part[w][i][lane];
-    const int m = i * 16 + l16, n = n0 + 4 * g;
-    if (m >= a.m) continue;
-    const float xs = a.x_scale[m];
+      for (int w = 1; w < NW; ++w) v += part[w][i][lane];
+      const int m = i * 16 + l16, n = n0 + 4 * g;
+      if (m >= a.m) continue;
+      const float xs = a.x_scale[m];
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (n + e < a.n)
-        out[(int64_t)m * a.o_ld + n + e] =
-            (TO)activate(fmaf((float)v[e], xs * a.w_scale[n + e], a.bias ? a.bias[n + e] : 0.f), a.act);
-  }
+      for (int e = 0; e < 4; ++e)
+        if (n + e < a.n)
+          out[(int64_t)m * a.o_ld + n + e] = (TO)activate<decltype(act)::value>(
+              fmaf((float)v[e], xs * a.w_scale[n + e], a.bias ? a.bias[n + e] : 0.f));
+    }
+  });
 }
 
-template <class TO, int WAN, int WAM, int GN, int GM>
+template <class TO, int WAN, int WAM, int GN, int GM, int BK, int OCC>
 void launch_tile(const LinArgs& a, bool dma, hipStream_t st) {
   constexpr int BN = WAN * GN * 64, BM = WAM * GM * 16, NT = WAN * WAM * 64;
   const dim3 grid((unsigned)((int64_t)((a.m + BM - 1) / BM) * ((a.n + BN - 1) / BN)));
-  if (dma) hipLaunchKernelGGL((tile_kernel<TO, WAN, WAM, GN, GM, true>), grid, dim3(NT), 0, st, a);
-  else hipLaunchKernelGGL((tile_kernel<TO, WAN, WAM, GN, GM, false>), grid, dim3(NT), 0, st, a);
+  if (dma) hipLaunchKernelGGL((tile_kernel<TO, WAN, WAM, GN, GM, BK, OCC, true>), grid, dim3(NT), 0, st, a);
+  else hipLaunchKernelGGL((tile_kernel<TO, WAN, WAM, GN, GM, BK, OCC, false>), grid, dim3(NT), 0, st, a);
 }
 
 template <class TO>
@@ -283,10 +293,17 @@ int launch_linear(const LinArgs& a, hipStream_t st) {
   const bool dma = a.k % 16 == 0 && a.x_ld % 16 == 0 && a.w_ld % 16 == 0 && (uintptr_t)a.x % 16 == 0 &&
                    (uintptr_t)a.w % 16 == 0;
   auto tiles = [&](int bm, int bn) { return (int64_t)((a.m + bm - 1) / bm) * ((a.n + bn - 1) / bn); };
-  // the largest tile that still gives every compute unit a workgroup
-  if (tiles(256, 256) >= 256) launch_tile<TO, 2, 4, 2, 4>(a, dma, st);
-  else if (tiles(128, 128) >= 256) launch_tile<TO, 2, 2, 1, 4>(a, dma, st);
-  else launch_tile<TO, 1, 4, 1, 1>(a, dma, st);
+  // The largest tile that still gives every compute unit a workgroup: operands are read from LDS 0.75 (256 x 256), 1
+  // (128 x 128) and 2.5 (64 x 64) times per 16-deep product.  Up to K = 512 a tile has so few steps that its
+  // epilogue and first loads take longer than its products: 128 x 128 in 64-byte steps leaves room for four workgroups
+  // a CU, which hide each other's.  Measured (us, fp16 out; 256 | 128 | 128 at 64 bytes | 64):
+  //   49662 x 512 x 2048 GELU 154 | 143 | 122 | 172    8192 x 4096 x 16384  502 | 575 | 675 | 878
+  //   4096 x 1024 x 4096       24 |  28 |  29 |  36    2048 x 2048 x 2048    30 |  16 |  20 |  18
+  //   777 x 1008 x 1537 GELU   25 |  12 |  14 | 8.8    128 x 4096 x 16384    50 |  27 |  37 |  20
+  if (a.k <= 512 && tiles(128, 128) >= 1024) launch_tile<TO, 2, 2, 1, 4, 64, 4>(a, dma, st);
+  else if (tiles(256, 256) >= 256) launch_tile<TO, 2, 4, 2, 4, 128, 2>(a, dma, st);
+  else if (tiles(128, 128) >= 256) launch_tile<TO, 2, 2, 1, 4, 128, 2>(a, dma, st);
+  else launch_tile<TO, 1, 4, 1, 1, 128, 2>(a, dma, st);
   SESA_CHECK_LAUNCH();
   return SESA_OK;
 }

@@ -211,8 +211,8 @@ def _norm_call(op, x, residual, gate, gate_act, post, post_weight, post_bias, sc
     rt = x.dtype if residual is None else residual.dtype
     xr = _rows(x)
     rr, gr = None if residual is None else _rows(residual), None if gate is None else _rows(gate)
-    y = x.new_empty(x.shape, dtype=rt)
-    n = x.new_empty(x.shape, dtype=torch.int8) if i8 else x.new_empty(x.shape)
+    y = torch.empty_like(x if residual is None else residual, memory_format=torch.contiguous_format)
+    n = torch.empty_like(x, dtype=torch.int8 if i8 else None, memory_format=torch.contiguous_format)
     qs = x.new_empty(x.shape[:-1], dtype=torch.float32) if i8 else None
     pw, pb = _param(op, "post_weight", post_weight, d), _param(op, "post_bias", post_bias, d)
     nw, nb = _param(op, "pre_weight", pre_weight, d), _param(op, "pre_bias", pre_bias, d)
@@ -261,7 +261,7 @@ def _quantize_i8(x):
     if x.dtype not in _DTYPE or x.dim() < 1:
         _fail(op, f"x: expected float32, float16 or bfloat16 [..., dim], got {x.dtype} {list(x.shape)}")
     xr = _rows(x)
-    q = x.new_empty(x.shape, dtype=torch.int8)
+    q = torch.empty_like(x, dtype=torch.int8, memory_format=torch.contiguous_format)
     s = x.new_empty(x.shape[:-1], dtype=torch.float32)
     a = N.SesaNormArgs(rows=xr.shape[0], dim=x.shape[-1], x_dtype=_DTYPE[x.dtype], r_dtype=_DTYPE[x.dtype],
                        x=xr.data_ptr(), x_ld=xr.stride(0), q=q.data_ptr(), q_ld=x.shape[-1], q_scale=s.data_ptr())
@@ -309,7 +309,7 @@ def _rope_axes(xs, positions, freqs, sections, layout):
         _fail("rope_axes", f"one or two tensors, got {len(xs)}")
     _device("rope_axes", xs[0])
     xs = [x if x.dim() < 1 or x.stride(-1) == 1 else x.contiguous() for x in xs]
-    outs = [x.new_empty(x.shape) for x in xs]
+    outs = [torch.empty_like(x, memory_format=torch.contiguous_format) for x in xs]
     _rope_call("rope_axes", xs, outs, positions, freqs, sections, layout)
     return outs
 
@@ -376,7 +376,7 @@ def _attn_call(op, q, k, v, cu, causal, scale, gate, out, zero_rest):
          "-> Tensor")
 def _attention_packed(q, k, v, cu_seqlens, causal, scale, gate):
     _device("attention_packed", q)
-    out = q.new_empty(q.shape)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     _attn_call("attention_packed", q, k, v, cu_seqlens, causal, scale, gate, out, True)
     return out
 
