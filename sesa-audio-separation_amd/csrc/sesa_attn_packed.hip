@@ -59,7 +59,8 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_packed_kernel(sesa_attn_args 
   constexpr int BQ = NW * 32, NTH = NW * 64, ROW = D * 2, IMG = kKeys * ROW, CH = D / 8, IT = kKeys * CH / NTH;
   constexpr float kLog2e = 1.4426950408889634f;
   __shared__ __attribute__((aligned(16))) char smem[4 * IMG];   // [stage][K, V], rows of D elements
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l32 = lane & 31, hl = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l32 = lane & 31, hl = lane >> 5;
   const int group = a.heads / a.kv_heads;
   // a die's workgroups: consecutive query heads and tiles of one (lane, key head), so its L2 holds that head's K and V
   int t = die_tile(blockIdx.x, gridDim.x);
@@ -108,6 +109,7 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_packed_kernel(sesa_attn_args 
   auto swz = [&](int row, int chunk) { return row * ROW + ((chunk ^ key_of(row)) << 4); };
   // DMA piece i of this wave: LDS bytes 1024 (wave + NW i) .. of an image, lane * 16 into it; the swizzle goes on the
   // source.  Offsets count from the block's first key.
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
   constexpr int PCS = IMG / 1024 / NW, RPP = 1024 / ROW;   // pieces per wave and image, rows per piece
   uint32_t koff[DMA ? PCS : 1], voff[DMA ? PCS : 1];
   auto offsets = [&](int n) {   // n: keys of the block that exist
@@ -119,16 +121,16 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_packed_kernel(sesa_attn_args 
     }
   };
   u32x4 kreg[DMA ? 1 : IT], vreg[DMA ? 1 : IT];
-  auto load_block = [&](int kb, char* stage) {
+  auto load_block = [&](int kb, int stage) {
     const int64_t p0 = (int64_t)start + kb * kKeys;
     if constexpr (DMA) {
       if (p0 + kKeys > end) offsets((int)(end - p0));
       const char* kb0 = reinterpret_cast<const char*>(kp + p0 * a.k_t);
       const char* vb0 = reinterpret_cast<const char*>(vp + p0 * a.v_t);
 #pragma unroll
-      for (int i = 0; i < PCS; ++i) dma16(kb0 + koff[i], stage + (wave + NW * i) * 1024);
+      for (int i = 0; i < PCS; ++i) dma16_asm(kb0, koff[i], lds0 + stage + (wave + NW * i) * 1024);
 #pragma unroll
-      for (int i = 0; i < PCS; ++i) dma16(vb0 + voff[i], stage + IMG + (wave + NW * i) * 1024);
+      for (int i = 0; i < PCS; ++i) dma16_asm(vb0, voff[i], lds0 + stage + IMG + (wave + NW * i) * 1024);
     } else {
 #pragma unroll
       for (int i = 0; i < IT; ++i) {
@@ -140,38 +142,51 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_packed_kernel(sesa_attn_args 
       }
     }
   };
-  auto store_block = [&](char* stage) {
+  auto store_block = [&](int stage) {
     if constexpr (!DMA) {
 #pragma unroll
       for (int i = 0; i < IT; ++i) {
         const int e = tid + i * NTH, off = swz(e / CH, e % CH);
-        *reinterpret_cast<u32x4*>(stage + off) = kreg[i];
-        *reinterpret_cast<u32x4*>(stage + IMG + off) = vreg[i];
+        *reinterpret_cast<u32x4*>(smem + stage + off) = kreg[i];
+        *reinterpret_cast<u32x4*>(smem + stage + IMG + off) = vreg[i];
       }
     }
   };
-  // V^T fragment (d-block db, keys 16 ks ..): lane half hl gets the keys 4 hl .. + 3 and 8 + 4 hl .. + 3 of its step,
-  // the order in which the score registers hold them
-  const int tg = lane >> 4, ti = lane & 15;
-  auto vt = [&](const char* V, int ks, int db) -> u32x4 {
-    typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
-    const int d = db * 32 + 16 * (tg & 1) + 4 * (ti & 3), key = 16 * ks + 4 * (tg >> 1) + (ti >> 2);
+  // Fragment addresses: a key block's K row 32 rb + l32 and V rows 16 ks + .. differ from the first ones' by whole
+  // multiples of 16 rows, which leave key_of alone, so one offset per chunk serves all of them.
+  // V^T (d-block db, keys 16 ks ..): lane half hl gets the keys 4 hl .. + 3 and 8 + 4 hl .. + 3 of its step, the order in
+  // which the score registers hold them.
+  typedef __attribute__((address_space(3))) char lds_char;
+  typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+  lds_char* const lds = (lds_char*)smem;
+  int ko[D / 16], vo[2][D / 32];
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks) ko[ks] = swz(l32, 2 * ks + hl);
+  {
+    const int tg = lane >> 4, ti = lane & 15, key = 4 * (tg >> 1) + (ti >> 2);
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db) {
+      const int d = db * 32 + 16 * (tg & 1) + 4 * (ti & 3);
+      vo[0][db] = IMG + swz(key, d >> 3) + ((d & 7) << 1);
+      vo[1][db] = IMG + swz(key + 8, d >> 3) + ((d & 7) << 1);
+    }
+  }
+  auto vt = [&](int stage, int ks, int db) -> u32x4 {   // (16-bit elements move through the read unchanged)
     const bf16x4 t0 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
-        (__attribute__((address_space(3))) bf16x4*)(V + swz(key, d >> 3) + ((d & 7) << 1)));
+        (__attribute__((address_space(3))) bf16x4*)(lds + stage + vo[0][db] + 16 * ROW * ks));
     const bf16x4 t1 = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
-        (__attribute__((address_space(3))) bf16x4*)(V + swz(key + 8, d >> 3) + ((d & 7) << 1)));
+        (__attribute__((address_space(3))) bf16x4*)(lds + stage + vo[1][db] + 16 * ROW * ks));
     return __builtin_bit_cast(u32x4, __builtin_shufflevector(t0, t1, 0, 1, 2, 3, 4, 5, 6, 7));
   };
 
   const int last = a.causal ? min(end, q0 + BQ) : end;   // keys from here on reach no query of the tile
   const int n_blocks = (last - start + kKeys - 1) / kKeys;
-  if constexpr (DMA) offsets(kKeys);
-  load_block(0, smem);
-  store_block(smem);
-  for (int kb = 0; kb < n_blocks; ++kb) {
-    const char* K = smem + (kb & 1) * 2 * IMG;
-    const char* V = K + IMG;
-    char* next = smem + ((kb + 1) & 1) * 2 * IMG;
+  // blocks all of whose keys every query of the tile sees
+  const int n_whole = (min(end, a.causal ? q0 + 1 : end) - start) / kKeys;
+
+  auto step = [&](int kb, auto masked) {
+    constexpr bool MASKED = decltype(masked)::value;
+    const int cur = (kb & 1) * 2 * IMG, next = ((kb + 1) & 1) * 2 * IMG;
     // this wave's part of block kb has landed; behind the barrier everyone's has, and everyone is done with block
     // kb - 1, whose place block kb + 1 takes
     if constexpr (DMA) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -180,36 +195,34 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_packed_kernel(sesa_attn_args 
     f32x16 s[2];
 #pragma unroll
     for (int rb = 0; rb < 2; ++rb) {
+      u32x4 kf[D / 16];
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) kf[ks] = *(__attribute__((address_space(3))) const u32x4*)(lds + cur + ko[ks] + rb * 32 * ROW);
+      __builtin_amdgcn_sched_barrier(0);   // all reads before the first product: one LDS round trip, not one a product
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[rb][r] = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) {
-        const u32x4 kf = *reinterpret_cast<const u32x4*>(K + swz(rb * 32 + l32, 2 * ks + hl));
-        s[rb] = mfma16<T>(kf, qf[ks], s[rb]);
-      }
+      for (int ks = 0; ks < D / 16; ++ks) s[rb] = mfma16<T>(kf[ks], qf[ks], s[rb]);
     }
-    const int key0 = start + kb * kKeys;
-    const bool masked = key0 + kKeys > end || (a.causal && key0 + kKeys - 1 > q0 + wave * 32);
-    const int64_t lim = a.causal ? min((int64_t)end - 1, q_pos) : (int64_t)end - 1;   // last key this query sees
-    if (masked) {
+    // last key of the block that this query sees, counted like the registers' keys (4 hl taken off)
+    const int lim = (int)min((int64_t)(end - 1), a.causal ? q_pos : (int64_t)(end - 1)) - (start + kb * kKeys) - 4 * hl;
+    if constexpr (MASKED) {
 #pragma unroll
       for (int rb = 0; rb < 2; ++rb)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int key = key0 + rb * 32 + (r & 3) + 8 * (r >> 2) + 4 * hl;
-          if (key > lim) s[rb][r] = -INFINITY;
-        }
+        for (int r = 0; r < 16; ++r)
+          if (rb * 32 + (r & 3) + 8 * (r >> 2) > lim) s[rb][r] = -INFINITY;
     }
     float top = -INFINITY;
 #pragma unroll
     for (int rb = 0; rb < 2; ++rb)
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[rb][r]);
-    top = fmaxf(top, __shfl_xor(top, 32));
+    top = max_halves(top);
     // The running maximum moves only when a block exceeds it by more than 2^8 in the exponential (P stays <= 256, in
     // range for fp16), so most blocks leave O alone.  Both halves of a query hold the same values, so they agree.
-    if ((top - m_run) * c > 8.f || (m_run == -INFINITY && top > -INFINITY)) {
-      const float alpha = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_run - top) * c);
+    if ((top - m_run) * c > 8.f) {
+      const float alpha = __builtin_amdgcn_exp2f((m_run - top) * c);   // (the first time: 0)
       l_run *= alpha;
 #pragma unroll
       for (int db = 0; db < D / 32; ++db)
@@ -218,63 +231,74 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_packed_kernel(sesa_attn_args 
       m_run = top;
     }
     const float mc = m_run == -INFINITY ? 0.f : m_run * c;   // (no finite score so far: every P is exp(-inf) = 0)
-    float sum = 0.f;
 #pragma unroll
     for (int rb = 0; rb < 2; ++rb)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const float p = __builtin_amdgcn_exp2f(fmaf(s[rb][r], c, -mc));
         s[rb][r] = p;
-        sum += p;
+        l_run += p;   // this half's keys; the halves join at the end
       }
-    l_run += sum + __shfl_xor(sum, 32);
-    // A masked block multiplies probabilities of 0 with the keys its rows do not see: harmless for finite v, but 0 * inf
-    // is NaN, so look for non-finite v there (exponent all ones) and take that block element by element if there is one.
-    uint32_t bad = 0;
-    constexpr uint32_t kExp = std::is_same<T, f16>::value ? 0x7c007c00u : 0x7f807f80u;
-    constexpr uint32_t kOne = std::is_same<T, f16>::value ? 0x04000400u : 0x00800080u;
-    if (masked) {
-      for (int e = lane; e < IMG / 16; e += 64) {
-        const u32x4 w = *reinterpret_cast<const u32x4*>(V + e * 16);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) bad |= (w[q] & kExp) + kOne;
-      }
-    }
-    if (__ballot((bad & 0x80008000u) != 0)) {
-      int hide = hl;   // (opaque: keeps this rare path's addresses out of the loop's registers)
-      asm volatile("" : "+v"(hide));
+    for (int ks = 0; ks < 4; ++ks) {
+      f32x16& sv = s[ks >> 1];
+      const int r0 = 8 * (ks & 1);
+      const u32x4 pf = {pack2t<T>(sv[r0], sv[r0 + 1]), pack2t<T>(sv[r0 + 2], sv[r0 + 3]), pack2t<T>(sv[r0 + 4], sv[r0 + 5]),
+                        pack2t<T>(sv[r0 + 6], sv[r0 + 7])};
+      u32x4 vf[D / 32];
 #pragma unroll
-      for (int rb = 0; rb < 2; ++rb)
+      for (int db = 0; db < D / 32; ++db) vf[db] = vt(cur, ks, db);
+      if constexpr (MASKED) {
+        // A masked block multiplies probabilities of 0 with the keys its rows do not see: harmless for finite v, but
+        // 0 * inf is NaN.  So look for non-finite v (exponent all ones); where there are any, their products with the
+        // rows that do see them are added one by one and the fragments go on with 0 in their place.
+        constexpr uint32_t kExp = std::is_same<T, f16>::value ? 0x7c007c00u : 0x7f807f80u;
+        constexpr uint32_t kOne = std::is_same<T, f16>::value ? 0x04000400u : 0x00800080u;
+        uint32_t bad = 0;
+#pragma unroll
+        for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) bad |= (vf[db][q] & kExp) + kOne;
+        if (__ballot((bad & 0x80008000u) != 0)) {
 #pragma unroll 1
-        for (int r = 0; r < 16; ++r) {
-          const float mine = s[rb][r];
-#pragma unroll 1
-          for (int half = 0; half < 2; ++half) {
-            const float p = __shfl(mine, l32 + 32 * half);
-            const int key = rb * 32 + (r & 3) + 8 * (r >> 2) + 4 * half;
-            if (key0 + key > lim) continue;
+          for (int j = 0; j < 16; ++j) {   // key 16 ks + j: register r of lane half (j >> 2) & 1
+            const int r = r0 + (j & 3) + 4 * (j >> 3), key = 16 * ks + j;
+            const float p = __shfl(sv[r], l32 + 32 * ((j >> 2) & 1));
+            const bool sees = key - 4 * hl <= lim;
 #pragma unroll
             for (int db = 0; db < D / 32; ++db)
 #pragma unroll
               for (int q = 0; q < 16; ++q) {
-                const int d = db * 32 + 8 * (q >> 2) + 4 * hide + (q & 3);
-                o[db][q] = fmaf(p, (float)*reinterpret_cast<const T*>(V + swz(key, d >> 3) + ((d & 7) << 1)), o[db][q]);
+                const int d = db * 32 + 8 * (q >> 2) + 4 * hl + (q & 3);
+                const float v = (float)*(__attribute__((address_space(3))) const T*)(lds + cur + IMG + swz(key, d >> 3) +
+                                                                                     ((d & 7) << 1));
+                const bool odd = (__builtin_bit_cast(uint32_t, v) & 0x7f800000u) == 0x7f800000u;
+                if (odd && sees) o[db][q] = fmaf(p, v, o[db][q]);
               }
           }
+#pragma unroll
+          for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const uint32_t w = vf[db][q], t = (((w & kExp) + kOne) >> 15) & 0x00010001u;   // 1 in a non-finite half
+              vf[db][q] = w & ~(t * 0xffffu);
+            }
         }
-    } else {
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        const f32x16& sv = s[ks >> 1];
-        const int r0 = 8 * (ks & 1);
-        const u32x4 pf = {pack2t<T>(sv[r0], sv[r0 + 1]), pack2t<T>(sv[r0 + 2], sv[r0 + 3]),
-                          pack2t<T>(sv[r0 + 4], sv[r0 + 5]), pack2t<T>(sv[r0 + 6], sv[r0 + 7])};
-#pragma unroll
-        for (int db = 0; db < D / 32; ++db) o[db] = mfma16<T>(vt(V, ks, db), pf, o[db]);
       }
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db) o[db] = mfma16<T>(vf[db], pf, o[db]);
     }
     if (kb + 1 < n_blocks) store_block(next);
-  }
+  };
+
+  if constexpr (DMA) offsets(min(kKeys, end - start));
+  load_block(0, 0);
+  store_block(0);
+  __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0), where the compiler sees it: no wait for Q inside the loop
+  int kb = 0;
+  for (; kb < n_whole; ++kb) step(kb, std::false_type{});
+  for (; kb < n_blocks; ++kb) step(kb, std::true_type{});
+  l_run += __shfl_xor(l_run, 32);
 
   if (!q_ok) return;
   float scale = 1.f / l_run;

@@ -47,9 +47,11 @@ __device__ __forceinline__ void load8(const T* p, int left, float (&v)[8]) {
   }
 }
 
+// two fp32 values rounded to nearest even in one 32-bit word (one v_cvt_pk on gfx950)
 template <class T>
 __device__ __forceinline__ uint32_t pack2t(float a, float b) {
-  return (uint32_t)__builtin_bit_cast(uint16_t, (T)a) | ((uint32_t)__builtin_bit_cast(uint16_t, (T)b) << 16);
+  typedef T t2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, t2));
 }
 
 template <class T>
@@ -78,6 +80,19 @@ __device__ __forceinline__ void store8(T* p, int left, const float (&v)[8]) {
 // inside a template's lambda the host pass drops the kernel's launch stub over the builtin.
 __device__ __forceinline__ void dma16(const void* src, char* base) {
   __builtin_amdgcn_global_load_lds(src, (__attribute__((address_space(3))) void*)base, 16, 0, 0);
+}
+
+// The same by an asm statement, for kernels that also use the transposing LDS reads: the compiler takes those for stores
+// too and would wait for every load in flight before each.  No registers are written; the kernel waits on vmcnt itself.
+__device__ __forceinline__ void dma16_asm(const void* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
+}
+
+// Larger of the two values that lanes l and l ^ 32 hold
+__device__ __forceinline__ float max_halves(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+  const uint32_t a = r[0], b = r[1];
+  return fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
 }
 
 __device__ __forceinline__ float sigmoid_f(float v) {
