@@ -3,7 +3,7 @@
 // One pass over the keys with a running maximum and sum (fp32).  S^T = K Q^T on v_mfma_*_32x32x16: a lane then holds
 // one query's scores, so the row statistics need a single exchange (the two lane halves), and the same registers,
 // rounded to the type, are the second operand of O^T += V^T P^T; V^T comes from LDS by transposing 16-bit reads.
-#include "sesa_tokens.hpp"
+#include "sesa_tokens.h"
 
 namespace sesa {
 namespace {
@@ -55,7 +55,7 @@ __device__ __forceinline__ bool find_tile(const sesa_attn_args& a, int slot, int
 // LDS stores; keys behind the sequence repeat its last one).  Otherwise through registers, zeros behind the sequence
 // and behind head_dim.
 template <class T, int D, int NW, bool DMA>
-__global__ void __launch_bounds__(NW * 64, 2) attn_packed_kernel(sesa_attn_args a, int n_slots) {
+__global__ void __launch_bounds__(NW * 64, D == 64 ? 3 : 2) attn_packed_kernel(sesa_attn_args a, int n_slots) {
   constexpr int BQ = NW * 32, NTH = NW * 64, ROW = D * 2, IMG = kKeys * ROW, CH = D / 8, IT = kKeys * CH / NTH;
   constexpr float kLog2e = 1.4426950408889634f;
   __shared__ __attribute__((aligned(16))) char smem[4 * IMG];   // [stage][K, V], rows of D elements

@@ -257,11 +257,18 @@ struct Param {
   bool set = false;
 };
 
+struct LinI8 {         // an 8-bit Linear: w[n][k] at w_off of the byte blob, scales and bias [n] in the float blob
+  int n = 0, k = 0;
+  int64_t w_off = 0, s_off = 0, b_off = -1;
+};
+
 struct Layer {         // one transformer layer (Attention + FeedForward)
   std::string prefix;  // layers.i.j.layers.l
   int time = 1;
   Gemm qkv, out, ff1, ff2;
   int64_t rope_off = 0;  // float2 offset into the rope blob
+  LinI8 qkv8, out8, ff18, ff28;   // SESA_PREC_I8
+  int64_t freq_off = 0;           // rotary frequencies in the float blob
 };
 
 }  // namespace
@@ -289,6 +296,8 @@ struct sesa_bsr {
   uint16_t* d_w = nullptr;
   float* d_bias = nullptr;
   float2* d_rope = nullptr;
+  int8_t* d_w8 = nullptr;   // SESA_PREC_I8: the layers' weights ...
+  float* d_f8 = nullptr;    // ... their scales, biases and rotary frequencies
   bool finalized = false;
 };
 
@@ -308,6 +317,55 @@ int add_param(sesa_bsr* m, const std::string& name, std::vector<int64_t> shape) 
 
 const std::vector<float>& P(sesa_bsr* m, const std::string& name) { return m->params[m->by_name.at(name)].host; }
 
+// One 8-bit Linear: every row (output channel) on its own scale max |w| / 127, rounded half to even.
+template <class RowFn>
+LinI8 pack_i8(int n, int k, RowFn row_val, std::vector<int8_t>& w8, std::vector<float>& f8) {
+  LinI8 l;
+  l.n = n;
+  l.k = k;
+  w8.resize((w8.size() + 255) / 256 * 256);   // rows at 16-byte addresses where k allows it
+  l.w_off = (int64_t)w8.size();
+  w8.resize(w8.size() + (size_t)n * k);
+  l.s_off = (int64_t)f8.size();
+  std::vector<float> row(k);
+  for (int r = 0; r < n; ++r) {
+    float top = 0.f;
+    for (int i = 0; i < k; ++i) {
+      row[i] = row_val(r, i);
+      top = std::max(top, std::fabs(row[i]));
+    }
+    const float inv = top > 0.f ? 127.f / top : 0.f;
+    for (int i = 0; i < k; ++i) w8[l.w_off + (int64_t)r * k + i] = (int8_t)std::nearbyint(row[i] * inv);
+    f8.push_back(top / 127.f);
+  }
+  return l;
+}
+
+// RMSNorm gammas folded into the following Linear, as in the other precisions; gates and q / k / v in one product.
+void pack_layer_i8(sesa_bsr* m, Layer& L, std::vector<int8_t>& w8, std::vector<float>& f8) {
+  const std::string& p = L.prefix;
+  const int dim = m->cfg.dim, inner = m->inner, ff = m->ff;
+  auto bias = [&](LinI8& l, int n, auto val) {
+    l.b_off = (int64_t)f8.size();
+    for (int i = 0; i < n; ++i) f8.push_back(val(i));
+  };
+  const auto &Wqkv = P(m, p + ".0.to_qkv.weight"), &Wg = P(m, p + ".0.to_gates.weight"), &bg = P(m, p + ".0.to_gates.bias");
+  const auto &ga = P(m, p + ".0.norm.gamma"), &Wo = P(m, p + ".0.to_out.0.weight"), &gf = P(m, p + ".1.net.0.gamma");
+  const auto &W1 = P(m, p + ".1.net.1.weight"), &b1 = P(m, p + ".1.net.1.bias"), &W2 = P(m, p + ".1.net.4.weight"),
+             &b2 = P(m, p + ".1.net.4.bias");
+  L.qkv8 = pack_i8(3 * inner + m->cfg.heads, dim, [&](int n, int k) {
+    return (n < 3 * inner ? Wqkv[(int64_t)n * dim + k] : Wg[(int64_t)(n - 3 * inner) * dim + k]) * ga[k];
+  }, w8, f8);
+  bias(L.qkv8, 3 * inner + m->cfg.heads, [&](int n) { return n < 3 * inner ? 0.f : bg[n - 3 * inner]; });
+  L.out8 = pack_i8(dim, inner, [&](int n, int k) { return Wo[(int64_t)n * inner + k]; }, w8, f8);
+  L.ff18 = pack_i8(ff, dim, [&](int n, int k) { return W1[(int64_t)n * dim + k] * gf[k]; }, w8, f8);
+  bias(L.ff18, ff, [&](int n) { return b1[n]; });
+  L.ff28 = pack_i8(dim, ff, [&](int n, int k) { return W2[(int64_t)n * ff + k]; }, w8, f8);
+  bias(L.ff28, dim, [&](int n) { return b2[n]; });
+  L.freq_off = (int64_t)f8.size();
+  const auto& fr = P(m, p + ".0.rotary_embed.freqs");
+  f8.insert(f8.end(), fr.begin(), fr.begin() + m->cfg.dim_head / 2);
+}
 
 }  // namespace
 }  // namespace sesa
@@ -328,7 +386,8 @@ extern "C" int sesa_bsr_create(const sesa_bsr_config* cfg, sesa_bsr** out) {
                "bsr: mask_estimator_depth 1..4");
   SESA_REQUIRE(!c.mel || (c.freq_indices && c.n_freq_indices > 0), SESA_ERR_INVALID, "bsr: mel needs freq_indices");
   SESA_REQUIRE(c.mel || c.mask_estimator_depth >= 2, SESA_ERR_INVALID, "bsr: BS-Roformer mask MLP needs depth >= 2");
-  SESA_REQUIRE(c.precision == SESA_PREC_BF16X3 || c.precision == SESA_PREC_BF16 || c.precision == SESA_PREC_F16,
+  SESA_REQUIRE(c.precision == SESA_PREC_BF16X3 || c.precision == SESA_PREC_BF16 || c.precision == SESA_PREC_F16 ||
+                   c.precision == SESA_PREC_I8,
                SESA_ERR_INVALID, "bsr: precision");
   sesa_bsr* m = new sesa_bsr();
   m->cfg = c;
@@ -459,7 +518,14 @@ extern "C" int sesa_bsr_finalize(sesa_bsr* m, void* stream) {
     g.o_off = (int64_t)b * dim;
     m->band.groups.push_back(g);
   }
+  std::vector<int8_t> w8;
+  std::vector<float> f8;
+  const bool i8 = c.precision == SESA_PREC_I8;
   for (auto& L : m->layers) {
+    if (i8) {
+      pack_layer_i8(m, L, w8, f8);
+      continue;
+    }
     const std::string& p = L.prefix;
     const auto& Wqkv = P(m, p + ".0.to_qkv.weight");
     const auto& Wg = P(m, p + ".0.to_gates.weight");
@@ -537,9 +603,17 @@ extern "C" int sesa_bsr_finalize(sesa_bsr* m, void* stream) {
   if (m->d_w) (void)hipFree(m->d_w);
   if (m->d_bias) (void)hipFree(m->d_bias);
   if (m->d_rope) (void)hipFree(m->d_rope);
+  if (m->d_w8) (void)hipFree(m->d_w8);
+  if (m->d_f8) (void)hipFree(m->d_f8);
   m->d_w = nullptr;
   m->d_bias = nullptr;
   m->d_rope = nullptr;
+  m->d_w8 = nullptr;
+  m->d_f8 = nullptr;
+  if (i8) {
+    SESA_REQUIRE(hipMalloc(&m->d_w8, w8.size()) == hipSuccess, SESA_ERR_NOMEM, "bsr finalize: hipMalloc weights");
+    SESA_REQUIRE(hipMalloc(&m->d_f8, f8.size() * 4) == hipSuccess, SESA_ERR_NOMEM, "bsr finalize: hipMalloc scales");
+  }
   SESA_REQUIRE(hipMalloc(&m->d_w, blob.size() * 2) == hipSuccess, SESA_ERR_NOMEM, "bsr finalize: hipMalloc weights");
   SESA_REQUIRE(hipMalloc(&m->d_bias, std::max<size_t>(bias.size(), 1) * 4) == hipSuccess, SESA_ERR_NOMEM,
                "bsr finalize: hipMalloc bias");
@@ -550,6 +624,10 @@ extern "C" int sesa_bsr_finalize(sesa_bsr* m, void* stream) {
   if (!bias.empty()) SESA_CHECK_HIP(hipMemcpyAsync(m->d_bias, bias.data(), bias.size() * 4, hipMemcpyHostToDevice, st));
   if (!rope.empty())
     SESA_CHECK_HIP(hipMemcpyAsync(m->d_rope, rope.data(), rope.size() * sizeof(float2), hipMemcpyHostToDevice, st));
+  if (i8) {
+    SESA_CHECK_HIP(hipMemcpyAsync(m->d_w8, w8.data(), w8.size(), hipMemcpyHostToDevice, st));
+    SESA_CHECK_HIP(hipMemcpyAsync(m->d_f8, f8.data(), f8.size() * 4, hipMemcpyHostToDevice, st));
+  }
   SESA_CHECK_HIP(hipStreamSynchronize(st));
   int rc = upload_groups(m->band);
   for (auto& g : m->mlp)
@@ -590,6 +668,7 @@ extern "C" int sesa_bsr_finalize(sesa_bsr* m, void* stream) {
     if (!rc) rc = up(&m->d_inv_idx, idx);
   }
   for (auto& L : m->layers) {
+    if (i8) break;
     if (!rc) rc = upload_groups(L.qkv);
     if (!rc) rc = upload_groups(L.out);
     if (!rc) rc = upload_groups(L.ff1);
@@ -606,7 +685,7 @@ extern "C" int sesa_bsr_finalize(sesa_bsr* m, void* stream) {
 namespace {
 
 struct Plan {
-  size_t spec, xg, x, xp, rsc, qkv, ao, h, h2, mask, maskg, frames, total;
+  size_t spec, xg, x, xp, rsc, qkv, ao, h, h2, mask, maskg, frames, q8, pos, total;
 };
 
 Plan plan(const sesa_bsr* m, int B) {
@@ -626,8 +705,18 @@ Plan plan(const sesa_bsr* m, int B) {
   p.mask = off; off += al((size_t)m->cfg.num_stems * B * m->T * m->feat);
   p.maskg = off; off += m->cfg.mel ? al((size_t)m->cfg.num_stems * B * m->T * m->gfeat) : 0;
   p.frames = off; off += al((size_t)B * m->cfg.num_stems * m->cfg.audio_channels * m->T * kN);
+  const bool i8 = m->cfg.precision == SESA_PREC_I8;
+  const size_t wide = (size_t)std::max(std::max(m->cfg.dim, m->inner), m->ff);
+  p.q8 = off; off += i8 ? al(((size_t)tok * wide + 3) / 4) : 0;   // the Linears' 8-bit rows
+  p.pos = off; off += i8 ? al((size_t)tok * 2) : 0;               // (frame, band) of every token
   p.total = off;
   return p;
+}
+
+// (frame, band) positions of the token rows (b, t, band)
+__global__ void token_positions_kernel(int64_t rows, int T, int nb, int2* __restrict__ pos) {
+  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (i < rows) pos[i] = make_int2((int)(i / nb % T), (int)(i % nb));
 }
 
 TokGemmArgs gemm_args(const sesa_bsr* m, const Gemm& gm, const float* x, int64_t x_ld, float* out, int64_t o_ld,
@@ -654,6 +743,141 @@ double gemm_flops(const Gemm& gm, int64_t M) {
   double f = 0;
   for (auto& g : gm.groups) f += 2.0 * (double)M * g.N * g.K;
   return f;
+}
+
+// whether layer li is the last of its (time / freq) transformer
+bool stack_end(const sesa_bsr* m, size_t li) {
+  if (li + 1 == m->layers.size()) return true;
+  const Layer &L = m->layers[li], &N = m->layers[li + 1];
+  return N.time != L.time ||
+         N.prefix.substr(0, N.prefix.find(".layers.")) != L.prefix.substr(0, L.prefix.find(".layers."));
+}
+
+// The transformer layers in 8 bits.  Per layer: the seam (X += the last block's output, RMSNorm, rows to 8 bits, one
+// pass) -> q | k | v | gates -> rotary on q and k by (frame, band) -> attention over frames (bands side by side) or over
+// bands -> rows to 8 bits -> to_out -> the seam -> FF1 + GELU -> rows to 8 bits -> FF2.  The residual stream X stays
+// fp32, what passes between the products is fp16.
+int layers_i8(const sesa_bsr* m, int B, char* ws, const Plan& pl, hipStream_t st) {
+  const sesa_bsr_config& c = m->cfg;
+  const int dim = c.dim, inner = m->inner, T = m->T, nb = m->nb, dh = c.dim_head;
+  const int64_t M = (int64_t)B * T * nb;
+  float* X = reinterpret_cast<float*>(ws + pl.x);
+  uint16_t* QKV = reinterpret_cast<uint16_t*>(ws + pl.qkv);
+  uint16_t* AO = reinterpret_cast<uint16_t*>(ws + pl.ao);
+  uint16_t* H = reinterpret_cast<uint16_t*>(ws + pl.h);
+  uint16_t* O = reinterpret_cast<uint16_t*>(ws + pl.xp);   // a block's output before it joins X
+  int8_t* Q8 = reinterpret_cast<int8_t*>(ws + pl.q8);
+  float* RS = reinterpret_cast<float*>(ws + pl.rsc);
+  int2* POS = reinterpret_cast<int2*>(ws + pl.pos);
+  hipLaunchKernelGGL(token_positions_kernel, dim3((unsigned)((M + 255) / 256)), dim3(256), 0, st, M, T, nb, POS);
+  SESA_CHECK_LAUNCH();
+  int rc = SESA_OK;
+  // rows x [M][d] (add: joined to X first) -> (norm) -> Q8; without to8 only X is written
+  auto rows8 = [&](const void* x, int x_dtype, int d, bool add, int norm, bool to8) {
+    if (rc) return;
+    sesa_norm_args a{};
+    a.rows = M;
+    a.dim = d;
+    a.x_dtype = x_dtype;
+    a.r_dtype = SESA_DTYPE_F32;
+    a.x = x;
+    a.x_ld = d;
+    a.post = SESA_NORM_NONE;
+    a.pre = norm;
+    a.eps = 1e-24f / (float)d;   // F.normalize * sqrt(d): max(||x||, 1e-12)
+    if (add) {
+      a.residual = X;
+      a.y = X;
+      a.r_ld = a.y_ld = d;
+    }
+    if (to8) {
+      a.q = Q8;
+      a.q_ld = d;
+      a.q_scale = RS;
+    }
+    void* t0 = profile_begin(st);
+    rc = sesa_norm_residual(&a, st);
+    profile_end(t0, st, SESA_KCLASS_ACT, (double)M * d * ((x_dtype ? 2.0 : 4.0) + (add ? 8.0 : 0.0) + (to8 ? 1.0 : 0.0)));
+  };
+  auto linear = [&](const LinI8& l, int act, uint16_t* out, int64_t o_ld) {
+    if (rc) return;
+    void* t0 = profile_begin(st);
+    rc = sesa_linear_i8(Q8, l.k, RS, m->d_w8 + l.w_off, l.k, m->d_f8 + l.s_off, l.b_off < 0 ? nullptr : m->d_f8 + l.b_off,
+                        act, M, l.n, l.k, out, SESA_DTYPE_F16, o_ld, st);
+    profile_end(t0, st, SESA_KCLASS_TOKGEMM, 2.0 * (double)M * l.n * l.k,
+                (double)M * (l.k + 2.0 * l.n) + (double)l.n * l.k);
+  };
+  bool pending = false;   // O waits to join X
+  for (size_t li = 0; li < m->layers.size() && !rc; ++li) {
+    const Layer& L = m->layers[li];
+    rows8(pending ? (const void*)O : X, pending ? SESA_DTYPE_F16 : SESA_DTYPE_F32, dim, pending, SESA_NORM_RMS, true);
+    linear(L.qkv8, SESA_ACT_NONE, QKV, m->qkv_ld);
+    if (!rc) {
+      sesa_rope_args r{};
+      r.tokens = M;
+      r.head_dim = dh;
+      r.dtype = SESA_DTYPE_F16;
+      r.layout = SESA_ROPE_PAIRS;
+      r.n_axes = 2;
+      r.sections[0] = L.time ? dh / 2 : 0;
+      r.sections[1] = L.time ? 0 : dh / 2;
+      r.positions = POS;
+      r.positions_ld = 2;
+      r.freqs = m->d_f8 + L.freq_off;
+      r.n_tensors = 2;
+      for (int k = 0; k < 2; ++k)
+        r.t[k] = sesa_rope_tensor{QKV + k * inner, m->qkv_ld, dh, QKV + k * inner, m->qkv_ld, dh, c.heads};
+      void* t0 = profile_begin(st);
+      rc = sesa_rope_axes(&r, st);
+      profile_end(t0, st, SESA_KCLASS_ACT, (double)M * inner * 8.0);
+    }
+    if (!rc) {
+      sesa_attn_args a{};
+      const int64_t ld = m->qkv_ld;
+      a.tokens = L.time ? (int64_t)B * T : M;
+      a.lanes = L.time ? nb : 1;
+      a.n_seq = L.time ? B : B * T;
+      a.heads = a.kv_heads = c.heads;
+      a.head_dim = dh;
+      a.dtype = SESA_DTYPE_F16;
+      a.q = QKV;
+      a.k = QKV + inner;
+      a.v = QKV + 2 * inner;
+      a.gate = QKV + 3 * inner;
+      a.q_t = a.k_t = a.v_t = a.g_t = L.time ? nb * ld : ld;
+      a.q_l = a.k_l = a.v_l = a.g_l = ld;
+      a.q_h = a.k_h = a.v_h = dh;
+      a.g_h = 1;
+      a.scale = 1.f / std::sqrt((float)dh);
+      a.out = AO;
+      a.o_t = L.time ? (int64_t)nb * inner : inner;
+      a.o_l = inner;
+      a.o_h = dh;
+      const double n = L.time ? T : nb;
+      void* t0 = profile_begin(st);
+      rc = sesa_attention_packed(&a, st);
+      profile_end(t0, st, SESA_KCLASS_ATTN, 4.0 * (double)M * c.heads * n * dh, (double)M * inner * 8.0 + 2.0 * M * c.heads);
+    }
+    rows8(AO, SESA_DTYPE_F16, inner, false, SESA_NORM_NONE, true);
+    linear(L.out8, SESA_ACT_NONE, O, dim);
+    rows8(O, SESA_DTYPE_F16, dim, true, SESA_NORM_RMS, true);
+    linear(L.ff18, SESA_ACT_GELU, H, m->ff);
+    rows8(H, SESA_DTYPE_F16, m->ff, false, SESA_NORM_NONE, true);
+    linear(L.ff28, SESA_ACT_NONE, O, dim);
+    pending = true;
+    const bool norm_here = c.mel && stack_end(m, li);
+    if (!rc && (norm_here || li + 1 == m->layers.size())) {   // Mel: Transformer.norm of the joined stream (:218, :226)
+      rows8(O, SESA_DTYPE_F16, dim, true, SESA_NORM_NONE, false);
+      pending = false;
+      if (norm_here && !rc) {
+        const std::string tp = L.prefix.substr(0, L.prefix.find(".layers."));
+        hipLaunchKernelGGL(rownorm_kernel, dim3((unsigned)((M + 3) / 4)), dim3(256), 0, st, X, M, dim,
+                           m->d_affine + m->norm_off.at(tp));
+        SESA_CHECK_LAUNCH();
+      }
+    }
+  }
+  return rc;
 }
 
 }  // namespace
@@ -762,7 +986,11 @@ extern "C" int sesa_bsr_forward(sesa_bsr* m, const float* x, int B, float* out, 
   // applies on load, at half the bytes written and read); SESA_BSR_QKV16=0: fp32 rows (A/B)
   static const bool qkv16_on = !(getenv("SESA_BSR_QKV16") && std::string(getenv("SESA_BSR_QKV16")) == "0");
   const bool q16 = f16 && qkv16_on && m->qkv_ld % 4 == 0 && c.dim_head % 8 == 0 && m->inner % 4 == 0;
-  for (size_t li = 0; li < m->layers.size(); ++li) {
+  if (c.precision == SESA_PREC_I8) {
+    rc = layers_i8(m, B, ws, pl, st);
+    if (rc) return rc;
+  }
+  for (size_t li = 0; li < m->layers.size() && c.precision != SESA_PREC_I8; ++li) {
     const Layer& L = m->layers[li];
     // attention: QKV + gates (RMSNorm, rotary on q/k)
     split_x();
@@ -845,10 +1073,7 @@ extern "C" int sesa_bsr_forward(sesa_bsr* m, const float* x, int B, float* out, 
     }
     if (rc) return rc;
     // Mel: Transformer.norm after the last layer of each (time / freq) transformer (:218, :226)
-    const bool stack_end = li + 1 == m->layers.size() || m->layers[li + 1].time != L.time ||
-                           m->layers[li + 1].prefix.substr(0, m->layers[li + 1].prefix.find(".layers.")) !=
-                               L.prefix.substr(0, L.prefix.find(".layers."));
-    if (c.mel && stack_end) {
+    if (c.mel && stack_end(m, li)) {
       const std::string tp = L.prefix.substr(0, L.prefix.find(".layers."));
       hipLaunchKernelGGL(rownorm_kernel, dim3((unsigned)((Mtok + 3) / 4)), dim3(256), 0, st, X, Mtok, dim,
                          m->d_affine + m->norm_off.at(tp));
@@ -907,6 +1132,8 @@ extern "C" int sesa_bsr_destroy(sesa_bsr* m) {
   if (m->d_w) (void)hipFree(m->d_w);
   if (m->d_bias) (void)hipFree(m->d_bias);
   if (m->d_rope) (void)hipFree(m->d_rope);
+  if (m->d_w8) (void)hipFree(m->d_w8);
+  if (m->d_f8) (void)hipFree(m->d_f8);
   auto fr = [](Gemm& g) {
     if (g.d_groups) (void)hipFree(g.d_groups);
   };

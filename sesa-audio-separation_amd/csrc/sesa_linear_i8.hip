@@ -7,7 +7,7 @@
 //  * tile_kernel: BM tokens x BN channels per workgroup, K in 128-byte steps through a ring of LDS stages.
 //  * few_kernel (m <= 64): 16 channels per workgroup, the waves split K and read both operands straight into the
 //    matrix instruction's registers; joined in LDS.
-#include "sesa_tokens.hpp"
+#include "sesa_tokens.h"
 
 namespace sesa {
 namespace {

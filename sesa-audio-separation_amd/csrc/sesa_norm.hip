@@ -1,10 +1,11 @@
 // sesa_norm_residual: y = residual + scale * gate_act(gate) * post_norm(x), n = pre_norm(y) (fp or 8 bits), one pass.
 //
 // Memory bound: x, residual (and a per-row gate) are read once, y and n written once, and every value of a row stays
-// in registers between the reductions.  One wave per row up to dim 1024 (no LDS, no barrier); 256 or 1024 threads per
-// row above.  Statistics are two-pass over the registers (mean, then squared deviations), so LayerNorm does not
+// in registers between the reductions.  One wave per row up to dim 1024 (no LDS, no barrier), 256 threads up to 4096,
+// 1024 above: a thread keeps at most 32 values and enough rows are in flight to cover the loads (16384 x 8192 bf16,
+// sandwich norms and gate: 334 us at 256 threads, 278 at 512, 275 at 1024; 16384 x 4096: 134, 139, -).  Statistics are two-pass over the registers (mean, then squared deviations), so LayerNorm does not
 // cancel.
-#include "sesa_tokens.hpp"
+#include "sesa_tokens.h"
 
 namespace sesa {
 namespace {
@@ -193,7 +194,7 @@ int launch_norm(const sesa_norm_args& a, hipStream_t st) {
   else if (a.dim <= 1024) go(integral_constant<int, 64>{}, integral_constant<int, 2>{});
   else if (a.dim <= 2048) go(integral_constant<int, 256>{}, integral_constant<int, 1>{});
   else if (a.dim <= 4096) go(integral_constant<int, 256>{}, integral_constant<int, 2>{});
-  else if (a.dim <= 8192) go(integral_constant<int, 256>{}, integral_constant<int, 4>{});
+  else if (a.dim <= 8192) go(integral_constant<int, 1024>{}, integral_constant<int, 1>{});
   else if (a.dim <= 16384) go(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
   else go(integral_constant<int, 1024>{}, integral_constant<int, 4>{});
   SESA_CHECK_LAUNCH();

@@ -6,7 +6,7 @@
 // so position * freq wraps modulo one turn in integer arithmetic: the phase is off by at most |position| 2^-54 turns
 // whatever the position is (an fp32 product is off by half a radian at position 10^7).  The phase's top 32 bits then go
 // to sin / cos as fp32 half-turns, off by at most 2^-25 of a half-turn.
-#include "sesa_tokens.hpp"
+#include "sesa_tokens.h"
 
 namespace sesa {
 namespace {

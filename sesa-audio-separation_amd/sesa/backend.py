@@ -42,11 +42,11 @@ class HipBackend:
         self.use_amp = False
         self.exec_batch = exec_batch
 
-    def optimize_model(self, model, example_input=None, use_amp=False, use_channels_last=True):
+    def optimize_model(self, model, example_input=None, use_amp=False, use_channels_last=True, precision=None):
         self.model = model.eval()
         self.use_amp = bool(use_amp)
         if hasattr(model, "set_precision"):
-            model.set_precision(getattr(model, "_amp_precision", "bf16") if self.use_amp else "bf16x3")
+            model.set_precision(precision or (getattr(model, "_amp_precision", "bf16") if self.use_amp else "bf16x3"))
         self.compiled_model = self.model
         return self.compiled_model
 
@@ -63,10 +63,11 @@ PyTorchBackend = HipBackend
 
 
 def create_inference_session(model, device="cuda:0", optimize_mode="default", enable_amp=False, enable_tf32=True,
-                             enable_cudnn_benchmark=True, exec_batch=None):
+                             enable_cudnn_benchmark=True, exec_batch=None, precision=None):
     """pytorch_backend.create_inference_session (:492-536).  NOTE: the default of ``enable_amp``
     is False here (parity precision); the reference CLI also passes False unless --enable_amp.
-    ``exec_batch`` None: planned per track (sesa.demix.plan_exec_batch)."""
+    ``exec_batch`` None: planned per track (sesa.demix.plan_exec_batch).  ``precision`` (MI355X only): one of the
+    model's precisions by name instead of enable_amp's choice, e.g. the Roformers' ``int8``."""
     be = HipBackend(device=device, optimize_mode=optimize_mode, exec_batch=exec_batch)
-    be.optimize_model(model, use_amp=enable_amp)
+    be.optimize_model(model, use_amp=enable_amp, precision=precision)
     return be

@@ -68,6 +68,9 @@ def build_parser():
     p.add_argument("--demud_phaseremix_inst", action="store_true")
     p.add_argument("--exec_batch", type=int, default=0,
                    help="chunks per native forward (MI355X only; 0 = planned from the model and free HBM)")
+    p.add_argument("--precision", type=str, default=None,
+                   help="the model's precision by name (MI355X only; e.g. int8 for the Roformers: 8-bit Linears, about "
+                        "1 %% error a layer); default: --enable_amp's choice")
     return p
 
 
@@ -160,7 +163,7 @@ def proc_folder(argv=None):
     backend = create_inference_session(model, device=device, optimize_mode=args.optimize_mode,
                                        enable_amp=args.enable_amp, enable_tf32=args.enable_tf32,
                                        enable_cudnn_benchmark=args.enable_cudnn_benchmark,
-                                       exec_batch=args.exec_batch or None)
+                                       exec_batch=args.exec_batch or None, precision=args.precision)
     print(f"Model load time: {time.time() - t0:.2f} sec")
     run_folder(backend, model, args, config, device)
     return 0

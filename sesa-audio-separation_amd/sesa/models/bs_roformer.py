@@ -32,9 +32,12 @@ class BSRoformer(NativeModule):
     _prefix = "bsr"
     # fp16: the QKV / FF Linears on one fp16 MFMA pass (include/sesa.h SESA_PREC_F16; 7e-6 emulated on the
     # full vocals chunk); the band split, attention, out-projection and mask MLPs stay bf16x3
-    _precisions = ("bf16x3", "bf16", "fp16")
+    # int8: those Linears on 8-bit integers (one scale per token and output channel), attention in fp16, built from the
+    # operators of sesa/token_ops.py (SESA_PREC_I8); opt-in, outside the 1e-4 RMS gate
+    _precisions = ("bf16x3", "bf16", "fp16", "int8")
     _amp_precision = "fp16"  # --enable_amp (the reference's AMP is fp16 autocast)
-    _prec_codes = {"bf16x3": N.SESA_PREC_BF16X3, "bf16": N.SESA_PREC_BF16, "fp16": N.SESA_PREC_F16}
+    _prec_codes = {"bf16x3": N.SESA_PREC_BF16X3, "bf16": N.SESA_PREC_BF16, "fp16": N.SESA_PREC_F16,
+                   "int8": N.SESA_PREC_I8}
 
     def __init__(self, dim, *, depth, stereo=False, num_stems=1, time_transformer_depth=2, freq_transformer_depth=2,
                  linear_transformer_depth=0, freqs_per_bands=DEFAULT_FREQS_PER_BANDS, dim_head=64, heads=8,
