@@ -71,15 +71,18 @@ __device__ __forceinline__ int key_w(int r) { return BK == 128 ? (r & 3) | ((r >
 // Channel order: accumulator block j (0..3) of a 64-channel group holds, in row 4 g + i of the matrix instruction,
 // channel 16 g + 4 j + i, so lane group g owns 16 consecutive channels (32 B of fp16 a lane, 128 B a token and
 // group) and the epilogue stores straight from registers.
-// DMA: rows 16-byte aligned and K % 16 == 0 -- stages filled by global_load_lds_dwordx4 (the swizzle on the source
-// address).  Otherwise through registers, where the last partial piece of a row is completed with zeros.
-template <class TO, int WAN, int WAM, int GN, int GM, int BK, int OCC, bool DMA>
+// DMA: rows 16-byte aligned and K % 16 == 0 -- a ring of S stages filled by global_load_lds_dwordx4 (the swizzle on the
+// source address), S - 1 of them in flight.  Otherwise two stages filled through S - 1 sets of registers, where the last
+// partial piece of a row is completed with zeros.
+template <class TO, int WAN, int WAM, int GN, int GM, int BK, int S, int OCC, bool DMA>
 __global__ void __launch_bounds__(WAN* WAM * 64, OCC) tile_kernel(LinArgs a) {
   constexpr int NW = WAN * WAM, BN = WAN * GN * 64, BM = WAM * GM * 16;
   constexpr int STAGE = (BN + BM) * BK, PIECES = STAGE / 1024 / NW, WP = BN * BK / 1024 / NW;   // per wave
   constexpr int LPR = BK / 16, RPP = 64 / LPR;   // lanes per row, rows per piece
   static_assert(STAGE % (1024 * NW) == 0 && BN * BK % (1024 * NW) == 0, "whole pieces per wave");
-  __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];
+  constexpr int SLOTS = DMA ? S : 2;
+  static_assert(S >= 2 && S <= 4 && 2 * PIECES <= 63, "counted waits");
+  __shared__ __attribute__((aligned(16))) char smem[SLOTS * STAGE];
   float* xs_l = reinterpret_cast<float*>(smem);   // the tile's scales and bias, once the stages are done
   float* ws_l = xs_l + BM;
   float* b_l = ws_l + BN;
@@ -104,56 +107,71 @@ __global__ void __launch_bounds__(WAN* WAM * 64, OCC) tile_kernel(LinArgs a) {
     piece[p] = 16 * (lane % LPR ^ (is_w ? key_w<BK>(r) : key_x<BK>(r)));
     src[p] = is_w ? a.w + (int64_t)min(n0 + r, a.n - 1) * a.w_ld : a.x + (int64_t)min(m0 + r, a.m - 1) * a.x_ld;
   }
-  u32x4 held[DMA ? 1 : PIECES];
+  constexpr int SETS = DMA ? 1 : S - 1;
+  u32x4 held[SETS][DMA ? 1 : PIECES];
   auto lds_at = [&](int p) { return (p < WP ? 0 : BN * BK) + (wave + NW * (p < WP ? p : p - WP)) * 1024; };
-  auto fetch = [&](int s, char* stage) {
+  auto fetch = [&](int s, char* stage, u32x4* set) {
+    const bool whole = (s + 1) * BK <= a.k;
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
       const int k = s * BK + piece[p];
-      if constexpr (DMA) {   // pieces past K: any valid address (their products are masked in the last step)
-        dma16(src[p] + (k < a.k ? k : 0), stage + lds_at(p));
-      } else {
-        held[p] = __builtin_bit_cast(u32x4, load_k(src[p], k, a.k));
-      }
+      if constexpr (DMA)   // pieces past K: any valid address (their products are masked in the last step)
+        dma16(src[p] + (whole || k < a.k ? k : 0), stage + lds_at(p));
+      else
+        set[p] = whole ? load16(src[p] + k) : __builtin_bit_cast(u32x4, load_k(src[p], k, a.k));
     }
   };
-  auto put = [&](char* stage) {
+  auto put = [&](char* stage, const u32x4* set) {
     if constexpr (!DMA) {
 #pragma unroll
-      for (int p = 0; p < PIECES; ++p) *reinterpret_cast<u32x4*>(stage + lds_at(p) + lane * 16) = held[p];
+      for (int p = 0; p < PIECES; ++p) *reinterpret_cast<u32x4*>(stage + lds_at(p) + lane * 16) = set[p];
     }
   };
 
   i32x4 acc[GN][4][GM];
   const int l16 = lane & 15, g = lane >> 4;
+  // All fragment reads of ONCE 64-byte halves stand before their products: left to itself the compiler reuses one
+  // register set and waits out an LDS round trip per product, which a small tile has no other waves to hide.
+  constexpr int HALVES = BK / 64, ONCE = GN * GM <= 4 ? HALVES : 1;
   auto compute = [&](const char* stage, int s) {
 #pragma unroll
-    for (int h = 0; h < BK / 64; ++h) {
-      const int k0 = s * BK + h * 64;
-      if (k0 >= a.k) break;
-      i32x4 wf[GN][4], xf[GM];
+    for (int h0 = 0; h0 < HALVES; h0 += ONCE) {
+      i32x4 wf[ONCE][GN][4], xf[ONCE][GM];
 #pragma unroll
-      for (int i = 0; i < GM; ++i) {
-        const int r = (wm * GM + i) * 16 + l16;
-        xf[i] = *reinterpret_cast<const i32x4*>(stage + BN * BK + r * BK + 16 * ((h * 4 + g) ^ key_x<BK>(r)));
-      }
+      for (int q = 0; q < ONCE; ++q) {
+        const int h = h0 + q;
 #pragma unroll
-      for (int u = 0; u < GN; ++u)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int r = (wn * GN + u) * 64 + (l16 >> 2) * 16 + j * 4 + (l16 & 3);
-          wf[u][j] = *reinterpret_cast<const i32x4*>(stage + r * BK + 16 * ((h * 4 + g) ^ key_w<BK>(r)));
+        for (int i = 0; i < GM; ++i) {
+          const int r = (wm * GM + i) * 16 + l16;
+          xf[q][i] = *reinterpret_cast<const i32x4*>(stage + BN * BK + r * BK + 16 * ((h * 4 + g) ^ key_x<BK>(r)));
         }
-      if (DMA && k0 + 64 > a.k && k0 + 16 * g >= a.k) {   // (K % 16 == 0: whole pieces lie inside or outside)
-#pragma unroll
-        for (int i = 0; i < GM; ++i) xf[i] = i32x4{0, 0, 0, 0};
-      }
-#pragma unroll
-      for (int i = 0; i < GM; ++i)
 #pragma unroll
         for (int u = 0; u < GN; ++u)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) acc[u][j][i] = mfma_i8(wf[u][j], xf[i], acc[u][j][i]);
+          for (int j = 0; j < 4; ++j) {
+            const int r = (wn * GN + u) * 64 + (l16 >> 2) * 16 + j * 4 + (l16 & 3);
+            wf[q][u][j] = *reinterpret_cast<const i32x4*>(stage + r * BK + 16 * ((h * 4 + g) ^ key_w<BK>(r)));
+          }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int q = 0; q < ONCE; ++q) {
+        // the last step: pieces from K on hold anything (DMA; K % 16 == 0, so they lie whole inside or outside)
+        const int k0 = s * BK + (h0 + q) * 64;
+        if (DMA && k0 + 64 > a.k) {
+          const bool out = k0 + 16 * g >= a.k;
+#pragma unroll
+          for (int i = 0; i < GM; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) xf[q][i][e] = out ? 0 : xf[q][i][e];
+        }
+#pragma unroll
+        for (int i = 0; i < GM; ++i)
+#pragma unroll
+          for (int u = 0; u < GN; ++u)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[u][j][i] = mfma_i8(wf[q][u][j], xf[q][i], acc[u][j][i]);
+      }
     }
   };
 
@@ -163,18 +181,42 @@ __global__ void __launch_bounds__(WAN* WAM * 64, OCC) tile_kernel(LinArgs a) {
     for (int j = 0; j < 4; ++j)
 #pragma unroll
       for (int i = 0; i < GM; ++i) acc[u][j][i] = i32x4{0, 0, 0, 0};
-  fetch(0, smem);
-  put(smem);
-  for (int s = 0; s < steps; ++s) {
-    char* cur = smem + (s & 1) * STAGE;
-    char* next = smem + ((s + 1) & 1) * STAGE;
-    // this wave's part of stage s has landed; behind the barrier everyone's has, and everyone is done with stage s - 1,
-    // whose place stage s + 1 takes
-    if constexpr (DMA) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    sesa_sync();
-    if (s + 1 < steps) fetch(s + 1, next);
-    compute(cur, s);
-    if (s + 1 < steps) put(next);
+  if constexpr (DMA) {
+#pragma unroll
+    for (int s = 0; s < S - 1; ++s)
+      if (s < steps) fetch(s, smem + s * STAGE, nullptr);
+    int slot = 0;
+    for (int s = 0; s < steps; ++s) {
+      // this wave's part of stage s has landed (at most the pieces of the stages behind it are on the way); behind the
+      // barrier everyone's has, and everyone is done with stage s - 1, whose slot stage s + S - 1 takes
+      const int behind = min(S - 2, steps - 1 - s);
+      if (S > 3 && behind == 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PIECES) : "memory");
+      else if (S > 2 && behind == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PIECES) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      stage_sync();
+      const int ahead = slot ? slot - 1 : S - 1;   // (slot + S - 1) % S
+      if (s + S - 1 < steps) fetch(s + S - 1, smem + ahead * STAGE, nullptr);
+      compute(smem + slot * STAGE, s);
+      slot = slot + 1 < S ? slot + 1 : 0;
+    }
+  } else {
+    // stage s + 1 waits in registers while stage s is computed, and goes to the other slot behind it; set j holds the
+    // stages j, j + SETS, ...
+#pragma unroll
+    for (int j = 0; j < SETS; ++j)
+      if (j < steps) fetch(j, nullptr, held[j]);
+    put(smem, held[0]);
+    for (int s0 = 0; s0 < steps; s0 += SETS) {
+#pragma unroll
+      for (int j = 0; j < SETS; ++j) {
+        const int s = s0 + j;
+        if (s >= steps) break;
+        stage_sync();
+        if (s + SETS < steps) fetch(s + SETS, nullptr, held[j]);
+        compute(smem + (s & 1) * STAGE, s);
+        if (s + 1 < steps) put(smem + ((s + 1) & 1) * STAGE, held[(j + 1) % SETS]);
+      }
+    }
   }
 
   sesa_sync();
@@ -272,12 +314,12 @@ __global__ void __launch_bounds__(256) few_kernel(LinArgs a) {
   });
 }
 
-template <class TO, int WAN, int WAM, int GN, int GM, int BK, int OCC>
+template <class TO, int WAN, int WAM, int GN, int GM, int BK, int S, int OCC>
 void launch_tile(const LinArgs& a, bool dma, hipStream_t st) {
   constexpr int BN = WAN * GN * 64, BM = WAM * GM * 16, NT = WAN * WAM * 64;
   const dim3 grid((unsigned)((int64_t)((a.m + BM - 1) / BM) * ((a.n + BN - 1) / BN)));
-  if (dma) hipLaunchKernelGGL((tile_kernel<TO, WAN, WAM, GN, GM, BK, OCC, true>), grid, dim3(NT), 0, st, a);
-  else hipLaunchKernelGGL((tile_kernel<TO, WAN, WAM, GN, GM, BK, OCC, false>), grid, dim3(NT), 0, st, a);
+  if (dma) hipLaunchKernelGGL((tile_kernel<TO, WAN, WAM, GN, GM, BK, S, OCC, true>), grid, dim3(NT), 0, st, a);
+  else hipLaunchKernelGGL((tile_kernel<TO, WAN, WAM, GN, GM, BK, S, OCC, false>), grid, dim3(NT), 0, st, a);
 }
 
 template <class TO>
@@ -295,15 +337,17 @@ int launch_linear(const LinArgs& a, hipStream_t st) {
   auto tiles = [&](int bm, int bn) { return (int64_t)((a.m + bm - 1) / bm) * ((a.n + bn - 1) / bn); };
   // The largest tile that still gives every compute unit a workgroup: operands are read from LDS 0.75 (256 x 256), 1
   // (128 x 128) and 2.5 (64 x 64) times per 16-deep product.  Up to K = 512 a tile has so few steps that its
-  // epilogue and first loads take longer than its products: 128 x 128 in 64-byte steps leaves room for four workgroups
+  // epilogue and first loads take longer than its products: 128 x 128 in 64-byte steps leaves room for more workgroups
   // a CU, which hide each other's.  Measured (us, fp16 out; 256 | 128 | 128 at 64 bytes | 64):
-  //   49662 x 512 x 2048 GELU 154 | 143 | 122 | 172    8192 x 4096 x 16384  502 | 575 | 675 | 878
-  //   4096 x 1024 x 4096       24 |  28 |  29 |  36    2048 x 2048 x 2048    30 |  16 |  20 |  18
-  //   777 x 1008 x 1537 GELU   25 |  12 |  14 | 8.8    128 x 4096 x 16384    50 |  27 |  37 |  20
-  if (a.k <= 512 && tiles(128, 128) >= 1024) launch_tile<TO, 2, 2, 1, 4, 64, 4>(a, dma, st);
-  else if (tiles(256, 256) >= 256) launch_tile<TO, 2, 4, 2, 4, 128, 2>(a, dma, st);
-  else if (tiles(128, 128) >= 256) launch_tile<TO, 2, 2, 1, 4, 128, 2>(a, dma, st);
-  else launch_tile<TO, 1, 4, 1, 1, 128, 2>(a, dma, st);
+  //   49662 x 512 x 2048 GELU 154 | 143 | 119 | 172    8192 x 4096 x 16384  495 | 575 | 675 | 878
+  //   4096 x 1024 x 4096       22 |  28 |  29 |  36    2048 x 2048 x 2048    30 |  15 |  20 |  18
+  //   777 x 1008 x 1537 GELU   25 |  12 |  14 | 9.4    256 x 4096 x 4096     51 |  24 |  33 |  17
+  // The large ones run at the rate the chip sustains on int8 products (8192^3: 2.38 PFLOP/s; MFMA busy 49 % of the
+  // cycles at about 2.06 GHz); a ring deeper than two stages helps only the 64 x 64 tile (19 -> 17 us at 256 x 4096^2).
+  if (a.k <= 512 && tiles(128, 128) >= 1024) launch_tile<TO, 2, 2, 1, 4, 64, 2, 3>(a, dma, st);
+  else if (tiles(256, 256) >= 256) launch_tile<TO, 2, 4, 2, 4, 128, 2, 2>(a, dma, st);
+  else if (tiles(128, 128) >= 256) launch_tile<TO, 2, 2, 1, 4, 128, 2, 2>(a, dma, st);
+  else launch_tile<TO, 1, 4, 1, 1, 128, 4, 2>(a, dma, st);
   SESA_CHECK_LAUNCH();
   return SESA_OK;
 }

@@ -88,6 +88,14 @@ __device__ __forceinline__ void dma16_asm(const void* base, uint32_t off, uint32
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
 }
 
+// Workgroup barrier behind this wave's own LDS operations that leaves loads to LDS in flight: __syncthreads() would wait
+// for all of them, whatever stage they are for.  A kernel that uses it waits on vmcnt for the stage it is about to read.
+__device__ __forceinline__ void stage_sync() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 // Larger of the two values that lanes l and l ^ 32 hold
 __device__ __forceinline__ float max_halves(float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
