@@ -55,7 +55,7 @@ __device__ __forceinline__ bool find_tile(const sesa_attn_args& a, int slot, int
 // LDS stores; keys behind the sequence repeat its last one).  Otherwise through registers, zeros behind the sequence
 // and behind head_dim.
 template <class T, int D, int NW, bool DMA>
-__global__ void __launch_bounds__(NW * 64, D == 64 ? 3 : 2) attn_packed_kernel(sesa_attn_args a, int n_slots) {
+__global__ void __launch_bounds__(NW * 64, D == 64 ? (DMA ? 4 : 3) : 2) attn_packed_kernel(sesa_attn_args a, int n_slots) {
   constexpr int BQ = NW * 32, NTH = NW * 64, ROW = D * 2, IMG = kKeys * ROW, CH = D / 8, IT = kKeys * CH / NTH;
   constexpr float kLog2e = 1.4426950408889634f;
   __shared__ __attribute__((aligned(16))) char smem[4 * IMG];   // [stage][K, V], rows of D elements
@@ -184,6 +184,7 @@ __global__ void __launch_bounds__(NW * 64, D == 64 ? 3 : 2) attn_packed_kernel(s
   // blocks all of whose keys every query of the tile sees
   const int n_whole = (min(end, a.causal ? q0 + 1 : end) - start) / kKeys;
 
+  uint32_t bad = 0;   // bits 15 and 31: a non-finite v in a masked block
   auto step = [&](int kb, auto masked) {
     constexpr bool MASKED = decltype(masked)::value;
     const int cur = (kb & 1) * 2 * IMG, next = ((kb + 1) & 1) * 2 * IMG;
@@ -250,40 +251,13 @@ __global__ void __launch_bounds__(NW * 64, D == 64 ? 3 : 2) attn_packed_kernel(s
       for (int db = 0; db < D / 32; ++db) vf[db] = vt(cur, ks, db);
       if constexpr (MASKED) {
         // A masked block multiplies probabilities of 0 with the keys its rows do not see: harmless for finite v, but
-        // 0 * inf is NaN.  So look for non-finite v (exponent all ones); where there are any, their products with the
-        // rows that do see them are added one by one and the fragments go on with 0 in their place.
+        // 0 * inf is NaN.  So look for non-finite v (exponent all ones); a wave that meets any starts over below.
         constexpr uint32_t kExp = std::is_same<T, f16>::value ? 0x7c007c00u : 0x7f807f80u;
         constexpr uint32_t kOne = std::is_same<T, f16>::value ? 0x04000400u : 0x00800080u;
-        uint32_t bad = 0;
 #pragma unroll
         for (int db = 0; db < D / 32; ++db)
 #pragma unroll
           for (int q = 0; q < 4; ++q) bad |= (vf[db][q] & kExp) + kOne;
-        if (__ballot((bad & 0x80008000u) != 0)) {
-#pragma unroll 1
-          for (int j = 0; j < 16; ++j) {   // key 16 ks + j: register r of lane half (j >> 2) & 1
-            const int r = r0 + (j & 3) + 4 * (j >> 3), key = 16 * ks + j;
-            const float p = __shfl(sv[r], l32 + 32 * ((j >> 2) & 1));
-            const bool sees = key - 4 * hl <= lim;
-#pragma unroll
-            for (int db = 0; db < D / 32; ++db)
-#pragma unroll
-              for (int q = 0; q < 16; ++q) {
-                const int d = db * 32 + 8 * (q >> 2) + 4 * hl + (q & 3);
-                const float v = (float)*(__attribute__((address_space(3))) const T*)(lds + cur + IMG + swz(key, d >> 3) +
-                                                                                     ((d & 7) << 1));
-                const bool odd = (__builtin_bit_cast(uint32_t, v) & 0x7f800000u) == 0x7f800000u;
-                if (odd && sees) o[db][q] = fmaf(p, v, o[db][q]);
-              }
-          }
-#pragma unroll
-          for (int db = 0; db < D / 32; ++db)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const uint32_t w = vf[db][q], t = (((w & kExp) + kOne) >> 15) & 0x00010001u;   // 1 in a non-finite half
-              vf[db][q] = w & ~(t * 0xffffu);
-            }
-        }
       }
 #pragma unroll
       for (int db = 0; db < D / 32; ++db) o[db] = mfma16<T>(vf[db], pf, o[db]);
@@ -299,6 +273,48 @@ __global__ void __launch_bounds__(NW * 64, D == 64 ? 3 : 2) attn_packed_kernel(s
   for (; kb < n_whole; ++kb) step(kb, std::false_type{});
   for (; kb < n_blocks; ++kb) step(kb, std::true_type{});
   l_run += __shfl_xor(l_run, 32);
+
+  if (__ballot((bad & 0x80008000u) != 0)) {
+    // Rare: the wave's queries key by key, each only with the keys it sees, from global memory and without matrix
+    // instructions (no barrier: the waves of the tile may differ).  A lane half has its half of q's and o's elements.
+    const int64_t lim = min((int64_t)(end - 1), a.causal ? q_pos : (int64_t)(end - 1));
+    m_run = -INFINITY;
+    l_run = 0.f;
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[db][r] = 0.f;
+#pragma unroll 1
+    for (int64_t j = start; j < last; ++j) {
+      const T* kj = kp + j * a.k_t;
+      const T* vj = vp + j * a.v_t;
+      float dot = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        float kv[8];
+        load8(kj + 16 * ks + 8 * hl, hd - 16 * ks - 8 * hl, kv);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t w = qf[ks][e >> 1];
+          dot = fmaf((float)__builtin_bit_cast(T, (uint16_t)(e & 1 ? w >> 16 : w & 0xffffu)), kv[e], dot);
+        }
+      }
+      dot += __shfl_xor(dot, 32);
+      if (j > lim) continue;
+      const float top = fmaxf(m_run, dot);
+      const float base = top == -INFINITY ? 0.f : top * c;
+      const float alpha = __builtin_amdgcn_exp2f(fmaf(m_run, c, -base)), p = __builtin_amdgcn_exp2f(fmaf(dot, c, -base));
+      m_run = top;
+      l_run = fmaf(l_run, alpha, p);
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int d = db * 32 + 8 * (r >> 2) + 4 * hl + (r & 3);
+          o[db][r] = fmaf(p, d < hd ? (float)vj[d] : 0.f, o[db][r] * alpha);
+        }
+    }
+  }
 
   if (!q_ok) return;
   float scale = 1.f / l_run;

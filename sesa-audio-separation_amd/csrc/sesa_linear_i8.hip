@@ -32,7 +32,7 @@ __device__ __forceinline__ i32x4 mfma_i8(i32x4 a, i32x4 b, i32x4 c) {
 
 template <int ACT>
 __device__ __forceinline__ float activate(float v) {
-  if constexpr (ACT == SESA_ACT_GELU) return gelu_erf(v);
+  if constexpr (ACT == SESA_ACT_GELU) return gelu_f(v);
   if constexpr (ACT == SESA_ACT_TANH) return tanh_f(v);
   if constexpr (ACT == SESA_ACT_RELU) return v > 0.f || v != v ? v : 0.f;   // (keeps NaN)
   return v;

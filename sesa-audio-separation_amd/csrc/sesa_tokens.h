@@ -88,6 +88,22 @@ __device__ __forceinline__ void dma16_asm(const void* base, uint32_t off, uint32
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
 }
 
+// Exact (erf) GELU as max(v, 0) - |v| erfc(|v| / sqrt 2) / 2 -- both signs in one expression, no select --
+// with erfc(z) = t P4(t) exp(-z^2), t = 1 / (1 + p z) (Abramowitz & Stegun 7.1.26, |error| < 1.5e-7, the 1 / 2 in the
+// coefficients).  19 VALU slots where Phi(v) by a select takes 24: the 8-bit Linear's epilogue is bound by them.
+__device__ __forceinline__ float gelu_f(float v) {
+  const float z = fabsf(v);
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678118654752440f, z, 1.0f));
+  float p = 0.5f * 1.061405429f;
+  p = fmaf(p, t, 0.5f * -1.453152027f);
+  p = fmaf(p, t, 0.5f * 1.421413741f);
+  p = fmaf(p, t, 0.5f * -0.284496736f);
+  p = fmaf(p, t, 0.5f * 0.254829592f);
+  const float w = v * 0.84932180028801904272f;   // sqrt(log2(e) / 2): exp(-v^2 / 2) = exp2(-w^2)
+  const float q = p * t * __builtin_amdgcn_exp2f(-(w * w));
+  return fmaf(-fminf(z, 1e30f), q, fmaxf(v, 0.f));   // (the minimum: an infinity times its tail of 0)
+}
+
 // Workgroup barrier behind this wave's own LDS operations that leaves loads to LDS in flight: __syncthreads() would wait
 // for all of them, whatever stage they are for.  A kernel that uses it waits on vmcnt for the stage it is about to read.
 __device__ __forceinline__ void stage_sync() {
