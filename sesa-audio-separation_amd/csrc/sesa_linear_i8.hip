@@ -5,7 +5,7 @@
 //
 // Two kernels:
 //  * tile_kernel: BM tokens x BN channels per workgroup, K in 128-byte steps through a ring of LDS stages.
-//  * few_kernel (m <= 64): 16 channels per workgroup, the waves split K and read both operands straight into the
+//  * few_kernel (m <= 16, and to 64 with few channels): 16 channels per workgroup, the waves split K and read both operands straight into the
 //    matrix instruction's registers; joined in LDS.
 #include "sesa_tokens.h"
 
@@ -260,8 +260,8 @@ __global__ void __launch_bounds__(WAN* WAM * 64, OCC) tile_kernel(LinArgs a) {
 // Few tokens: bound by reading the weights once.  Workgroup = 16 channels x all (16 MI) tokens; NW waves take every
 // NW-th 64-byte step of K, kUnroll steps' loads in flight.
 template <class TO, int MI>
-__global__ void __launch_bounds__(256) few_kernel(LinArgs a) {
-  constexpr int NW = 4, U = MI == 1 ? 8 : 4;
+__global__ void __launch_bounds__(512) few_kernel(LinArgs a) {
+  constexpr int NW = 8, U = 4;   // (one token, 64 MB of weights: 17.0 us; 4 waves of 8 steps 17.9)
   __shared__ i32x4 part[NW][MI][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int l16 = lane & 15, g = lane >> 4;
@@ -282,7 +282,11 @@ __global__ void __launch_bounds__(256) few_kernel(LinArgs a) {
 #pragma unroll
     for (int q = 0; q < U; ++q)
 #pragma unroll
-      for (int i = 0; i < MI; ++i) xf[q][i] = __builtin_bit_cast(i32x4, load16(xr[i] + (s + q * NW) * 64));
+      for (int i = 0; i < MI; ++i) {
+        // up to 16 tokens: only the rows there are (repeats of the last one would cost as many loads as the weights)
+        if (MI > 1 || l16 < a.m) xf[q][i] = __builtin_bit_cast(i32x4, load16(xr[i] + (s + q * NW) * 64));
+        else xf[q][i] = i32x4{0, 0, 0, 0};
+      }
 #pragma unroll
     for (int q = 0; q < U; ++q)
 #pragma unroll
@@ -324,11 +328,14 @@ void launch_tile(const LinArgs& a, bool dma, hipStream_t st) {
 
 template <class TO>
 int launch_linear(const LinArgs& a, hipStream_t st) {
-  if (a.m <= 64) {
+  // Few tokens: the weights' reading counts, and splitting K over waves covers it.  From about 1536 blocks of 16 tokens x
+  // 16 channels on the same operands are re-read so often that the 64 x 64 tile takes less (us, few | tile, k = 4096:
+  // 17 x 8192 12.5 | 16.7, 17 x 16384 20.9 | 17.2, 32 x 8192 14.8 | 16.7, 64 x 4096 12.4 | 16.7, 64 x 8192 21.6 | 16.8).
+  if (a.m <= 16 || (a.m <= 64 && (int64_t)((a.m + 15) / 16) * ((a.n + 15) / 16) <= 1536)) {
     const dim3 grid((unsigned)((a.n + 15) / 16));
-    if (a.m <= 16) hipLaunchKernelGGL((few_kernel<TO, 1>), grid, dim3(256), 0, st, a);
-    else if (a.m <= 32) hipLaunchKernelGGL((few_kernel<TO, 2>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((few_kernel<TO, 4>), grid, dim3(256), 0, st, a);
+    if (a.m <= 16) hipLaunchKernelGGL((few_kernel<TO, 1>), grid, dim3(512), 0, st, a);
+    else if (a.m <= 32) hipLaunchKernelGGL((few_kernel<TO, 2>), grid, dim3(512), 0, st, a);
+    else hipLaunchKernelGGL((few_kernel<TO, 4>), grid, dim3(512), 0, st, a);
     SESA_CHECK_LAUNCH();
     return SESA_OK;
   }

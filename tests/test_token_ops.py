@@ -210,6 +210,16 @@ def test_linear_i8_shapes(m, k, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,k,n", [(17, 512, 12304), (33, 100, 8200), (64, 64, 6160), (64, 64, 6144), (16, 48, 30000), (70, 384, 256),
+                                   (8200, 320, 2064), (8200, 500, 2064)])
+def test_linear_i8_kernel_choice(m, k, n):
+    """Either side of the rules that choose between the kernels and tiles."""
+    from sesa import ops
+    x, xs, w, ws, b = linear_case(m + k + n, m, k, n)
+    linear_check(ops.linear_i8(x, xs, w, ws, b, out_dtype=torch.bfloat16), x, xs, w, ws, b)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("act", ["gelu", "tanh", "relu"])
 @pytest.mark.parametrize("m", [5, 200])
 def test_linear_i8_activations(act, m):
