@@ -308,6 +308,7 @@ int sesa_htdemucs_destroy(sesa_htdemucs* m);
  *   out[m, n] = act( x_scale[m] * w_scale[n] * sum_k x[m, k] * w[n, k] + bias[n] )
  * x [m, k] and w [n, k] int8, the sum in 32-bit integers (exact for k <= 131071, the largest accepted), the scales,
  * bias (nullable) and epilogue in fp32, out rounded once to out_dtype.  A scale that is NaN makes its row / column NaN.
+ * m < 2^31 - 256, n < 2^27.
  */
 int sesa_linear_i8(const int8_t* x, int64_t x_ld, const float* x_scale, const int8_t* w, int64_t w_ld,
                    const float* w_scale, const float* bias, int act, int64_t m, int n, int k, void* out, int out_dtype,
@@ -396,8 +397,9 @@ int sesa_rope_axes(const sesa_rope_args* args, void* stream);
 
 /* Softmax attention within each sequence of a packed run of tokens, grouped heads:
  *   out[i] = sigmoid(gate[i]) * sum_j softmax_j(scale * q[i] . k[j]) v[j],  j over i's own sequence (causal: j <= i)
- * Sequence s is tokens cu_seqlens[s] .. cu_seqlens[s + 1] - 1 (device int32 [n_seq + 1], non-decreasing; values
- * are held to [0, tokens] and to that order by the kernel); cu_seqlens NULL: n_seq sequences of tokens / n_seq.
+ * Sequence s is tokens cu_seqlens[s] .. cu_seqlens[s + 1] - 1 (device int32 [n_seq + 1], non-decreasing; the kernel
+ * holds values to [0, tokens], and values out of order give unspecified rows of out, never an access outside);
+ * cu_seqlens NULL: n_seq sequences of tokens / n_seq.
  * Tokens before cu_seqlens[0] and from cu_seqlens[n_seq] on belong to no sequence: their rows of out are left as
  * they were, or set to 0 with zero_rest.  `lanes` runs of the same lengths lie side by side (strides *_l).
  * head_dim a multiple of 8, 8..128; heads a multiple of kv_heads; fp16 or bf16.  Scores, softmax statistics and

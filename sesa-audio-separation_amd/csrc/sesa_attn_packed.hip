@@ -55,7 +55,7 @@ __device__ __forceinline__ bool find_tile(const sesa_attn_args& a, int slot, int
 // LDS stores; keys behind the sequence repeat its last one).  Otherwise through registers, zeros behind the sequence
 // and behind head_dim.
 template <class T, int D, int NW, bool DMA>
-__global__ void __launch_bounds__(NW * 64, D == 64 ? (DMA ? 4 : 3) : 2) attn_packed_kernel(sesa_attn_args a, int n_slots) {
+__global__ void __launch_bounds__(NW * 64, D == 64 ? (DMA ? 4 : 3) : 2) attn_packed_kernel(sesa_attn_args a, int n_slots, int n_blocks_all) {
   constexpr int BQ = NW * 32, NTH = NW * 64, ROW = D * 2, IMG = kKeys * ROW, CH = D / 8, IT = kKeys * CH / NTH;
   constexpr float kLog2e = 1.4426950408889634f;
   __shared__ __attribute__((aligned(16))) char smem[4 * IMG];   // [stage][K, V], rows of D elements
@@ -63,7 +63,8 @@ __global__ void __launch_bounds__(NW * 64, D == 64 ? (DMA ? 4 : 3) : 2) attn_pac
   const int l32 = lane & 31, hl = lane >> 5;
   const int group = a.heads / a.kv_heads;
   // a die's workgroups: consecutive query heads and tiles of one (lane, key head), so its L2 holds that head's K and V
-  int t = die_tile(blockIdx.x, gridDim.x);
+  if (long_block() >= n_blocks_all) return;
+  int t = die_tile((int)long_block(), n_blocks_all);
   const int gi = t % group;
   t /= group;
   const int slot = n_slots - 1 - t % n_slots;   // causal: the longest tiles first
@@ -343,13 +344,14 @@ int launch_attn(const sesa_attn_args& a, hipStream_t st) {
     return a.head_dim == D && strides % 8 == 0 && ((uintptr_t)a.k | (uintptr_t)a.v) % 16 == 0 && a.k_t >= 0 &&
            a.v_t >= 0 && a.k_t < (1 << 23) && a.v_t < (1 << 23);
   };
-  const dim3 grid((unsigned)blocks), block(NW * 64);
+  const dim3 grid = long_grid(blocks), block(NW * 64);
+  const int nb = (int)blocks;
   if (a.head_dim <= 64) {
-    if (dma(64)) hipLaunchKernelGGL((attn_packed_kernel<T, 64, NW, true>), grid, block, 0, st, a, (int)n_slots);
-    else hipLaunchKernelGGL((attn_packed_kernel<T, 64, NW, false>), grid, block, 0, st, a, (int)n_slots);
+    if (dma(64)) hipLaunchKernelGGL((attn_packed_kernel<T, 64, NW, true>), grid, block, 0, st, a, (int)n_slots, nb);
+    else hipLaunchKernelGGL((attn_packed_kernel<T, 64, NW, false>), grid, block, 0, st, a, (int)n_slots, nb);
   } else {
-    if (dma(128)) hipLaunchKernelGGL((attn_packed_kernel<T, 128, NW, true>), grid, block, 0, st, a, (int)n_slots);
-    else hipLaunchKernelGGL((attn_packed_kernel<T, 128, NW, false>), grid, block, 0, st, a, (int)n_slots);
+    if (dma(128)) hipLaunchKernelGGL((attn_packed_kernel<T, 128, NW, true>), grid, block, 0, st, a, (int)n_slots, nb);
+    else hipLaunchKernelGGL((attn_packed_kernel<T, 128, NW, false>), grid, block, 0, st, a, (int)n_slots, nb);
   }
   SESA_CHECK_LAUNCH();
   return SESA_OK;

@@ -368,8 +368,8 @@ extern "C" int sesa_linear_i8(const int8_t* x, int64_t x_ld, const float* x_scal
                               const float* w_scale, const float* bias, int act, int64_t m, int n, int k, void* out,
                               int out_dtype, int64_t o_ld, void* stream) {
   clear_error();
-  SESA_REQUIRE(m >= 0 && m < (1ll << 31) - 256 && n >= 1 && n < (1 << 30) && k >= 1 && k <= 131071, SESA_ERR_INVALID,
-               "linear_i8: m %lld, n %d, k %d (0 <= m < 2^31 - 256, 1 <= n < 2^30, 1 <= k <= 131071)", (long long)m, n, k);
+  SESA_REQUIRE(m >= 0 && m < (1ll << 31) - 256 && n >= 1 && n < (1 << 27) && k >= 1 && k <= 131071, SESA_ERR_INVALID,
+               "linear_i8: m %lld, n %d, k %d (0 <= m < 2^31 - 256, 1 <= n < 2^27, 1 <= k <= 131071)", (long long)m, n, k);
   SESA_REQUIRE(act >= SESA_ACT_NONE && act <= SESA_ACT_RELU, SESA_ERR_INVALID, "linear_i8: act %d", act);
   SESA_REQUIRE(out_dtype >= SESA_DTYPE_F32 && out_dtype <= SESA_DTYPE_BF16, SESA_ERR_INVALID, "linear_i8: out_dtype %d",
                out_dtype);

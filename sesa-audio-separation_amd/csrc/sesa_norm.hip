@@ -89,8 +89,8 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) norm_residual_kernel(se
   constexpr int RPB = TPR < 256 ? 256 / TPR : 1;
   __shared__ float red[TPR > 64 ? 5 * 16 : 1];
   const int t = threadIdx.x % TPR;
-  const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
-  if (row >= a.rows) return;   // (whole waves; with TPR > 64 the grid is exact, so every barrier is met)
+  const int64_t row = long_block() * RPB + threadIdx.x / TPR;
+  if (row >= a.rows) return;   // (whole waves; with TPR > 64 a block has one row, so its waves go together)
   const int dim = a.dim;
   float x[NCH][8], y[NCH][8], g[NCH][8];
   const TX* xr = reinterpret_cast<const TX*>(a.x) + row * a.x_ld;
@@ -187,7 +187,7 @@ int launch_norm(const sesa_norm_args& a, hipStream_t st) {
   auto go = [&](auto tpr, auto nch) {
     constexpr int TPR = decltype(tpr)::value, NCH = decltype(nch)::value, NT = TPR < 256 ? 256 : TPR;
     const int64_t blocks = (a.rows + NT / TPR - 1) / (NT / TPR);
-    hipLaunchKernelGGL((norm_residual_kernel<TX, TR, TPR, NCH>), dim3((unsigned)blocks), dim3(NT), 0, st, a);
+    hipLaunchKernelGGL((norm_residual_kernel<TX, TR, TPR, NCH>), long_grid(blocks), dim3(NT), 0, st, a);
   };
   using std::integral_constant;
   if (a.dim <= 512) go(integral_constant<int, 64>{}, integral_constant<int, 1>{});

@@ -23,7 +23,7 @@ struct RopePlan {
 template <class T, bool PAIRS>
 __global__ void __launch_bounds__(256) rope_axes_kernel(sesa_rope_args a, RopePlan pl) {
   const int64_t per_token = (int64_t)pl.n_all * pl.hsplit;
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t id = long_block() * 256 + threadIdx.x;
   const int64_t token = id / per_token;
   if (token >= a.tokens) return;
   const int rest = (int)(id - token * per_token);
@@ -101,11 +101,11 @@ __global__ void __launch_bounds__(256) rope_axes_kernel(sesa_rope_args a, RopePl
 template <class T>
 int launch_rope(const sesa_rope_args& a, const RopePlan& pl, hipStream_t st) {
   const int64_t blocks = (a.tokens * pl.n_all * pl.hsplit + 255) / 256;
-  SESA_REQUIRE(blocks < (1ll << 31), SESA_ERR_INVALID, "rope_axes: too many tokens");
+  SESA_REQUIRE(blocks < (1ll << 33), SESA_ERR_INVALID, "rope_axes: too many tokens");
   if (a.layout == SESA_ROPE_PAIRS)
-    hipLaunchKernelGGL((rope_axes_kernel<T, true>), dim3((unsigned)blocks), dim3(256), 0, st, a, pl);
+    hipLaunchKernelGGL((rope_axes_kernel<T, true>), long_grid(blocks), dim3(256), 0, st, a, pl);
   else
-    hipLaunchKernelGGL((rope_axes_kernel<T, false>), dim3((unsigned)blocks), dim3(256), 0, st, a, pl);
+    hipLaunchKernelGGL((rope_axes_kernel<T, false>), long_grid(blocks), dim3(256), 0, st, a, pl);
   SESA_CHECK_LAUNCH();
   return SESA_OK;
 }

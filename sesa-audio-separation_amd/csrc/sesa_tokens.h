@@ -85,7 +85,7 @@ __device__ __forceinline__ void dma16(const void* src, char* base) {
 // The same by an asm statement, for kernels that also use the transposing LDS reads: the compiler takes those for stores
 // too and would wait for every load in flight before each.  No registers are written; the kernel waits on vmcnt itself.
 __device__ __forceinline__ void dma16_asm(const void* base, uint32_t off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
 }
 
 // Exact (erf) GELU as max(v, 0) - |v| erfc(|v| / sqrt 2) / 2 -- both signs in one expression, no select --
@@ -130,6 +130,14 @@ __device__ __forceinline__ float tanh_f(float v) {
   const float small = v * fmaf(s, fmaf(s, fmaf(s, -17.f / 315.f, 2.f / 15.f), -1.f / 3.f), 1.f);
   return z < 0.09f ? small : big;
 }
+
+// A 1-D grid of nb workgroups as a launch takes it (a dimension holds less than 2^32 threads): rows of 2^18 workgroups,
+// and its workgroup number (nb and above: nothing to do).  The row length is a multiple of 8, so numbers keep their die.
+inline dim3 long_grid(int64_t nb) {
+  constexpr int64_t kRow = 1 << 18;
+  return nb <= kRow ? dim3((unsigned)nb) : dim3((unsigned)kRow, (unsigned)((nb + kRow - 1) / kRow));
+}
+__device__ __forceinline__ int64_t long_block() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
 
 // Tile order of a 1-D grid: workgroup b of nb runs on die b % 8, so give each die one contiguous range of tiles (its
 // own L2 then sees neighbouring tiles' operands).

@@ -175,6 +175,8 @@ def _(x, x_scale, weight, w_scale, bias, act, out_dtype):
 # ---- norm_residual --------------------------------------------------------------------------------------
 def _gate_groups(x, gate):
     """Rows of x per gate row: the gate has x's shape, or 1 in place of trailing leading dimensions of x."""
+    if not x.numel() and gate.shape == x.shape:
+        return 1
     lead, g = list(x.shape[:-1]), list(gate.shape[:-1])
     if gate.dim() == 2 and x.dim() == 2:   # [groups, dim] for flat rows
         if gate.shape[0] and x.shape[0] % gate.shape[0] == 0 and gate.shape[1] == x.shape[1]:
@@ -468,8 +470,9 @@ def attention_packed(q, k, v, cu_seqlens=None, *, causal=True, scale=None, gate=
     q [tokens, heads, head_dim], k and v [tokens, kv_heads, head_dim] (heads a multiple of kv_heads; head_dim a multiple of
     8 up to 128), fp16 or bf16, any strides with a contiguous last dimension.  A fourth dimension [tokens, lanes, ...]
     runs that many columns of the same lengths side by side (a Roformer's bands in its time attention).
-    cu_seqlens int32 [sequences + 1] on the device: sequence s is tokens cu_seqlens[s] .. cu_seqlens[s + 1] - 1 (None:
-    one sequence).  gate: logits [tokens, (lanes,) heads], a sigmoid on each head's output.  scale: head_dim ** -0.5.
+    cu_seqlens int32 [sequences + 1] on the device, non-decreasing: sequence s is tokens cu_seqlens[s] ..
+    cu_seqlens[s + 1] - 1 (None: one sequence).  It is read by the kernel and held to the run there: a boundary outside
+    is taken as the run's end, and boundaries out of order give unspecified rows, never an access outside.  gate: logits [tokens, (lanes,) heads], a sigmoid on each head's output.  scale: head_dim ** -0.5.
     Rows of no sequence (behind the last) come back 0; with ``out`` they are left as they were."""
     eager = _eager("attention_packed", q)
     if out is None:

@@ -793,3 +793,60 @@ def test_opcheck_token_ops():
     torch.library.opcheck(torch.ops.sesa.attention_packed.default, (q, k, v, None, True, None, None), test_utils=utils)
     torch.library.opcheck(torch.ops.sesa.attention_packed_into.default, (q, k, v, None, True, None, None, torch.zeros_like(q)),
                           test_utils=utils)
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """Rows so far apart that an element's offset passes 2^31 (and bytes 2^32): the last rows come out right."""
+    from sesa import ops
+    free, _ = torch.cuda.mem_get_info()
+    if free < 24 << 30:
+        pytest.skip("needs 24 GiB of device memory")
+    buf = torch.empty(6 << 30, dtype=torch.uint8, device="cuda")
+    g = gen(21)
+    m, ld = 70000, 65536                                     # 4.3 G elements of int8, rows 64 KiB apart
+    x = buf.view(torch.int8).as_strided((m, 64), (ld, 1))
+    x.copy_(torch.randint(-127, 128, (m, 64), generator=g, device="cuda", dtype=torch.int8))
+    w, ws = ops.quantize_i8(torch.randn(32, 64, generator=g, device="cuda"))
+    xs = torch.rand(m, generator=g, device="cuda")
+    linear_check(ops.linear_i8(x, xs, w, ws, out_dtype=torch.float32), x, xs, w, ws, None)
+    t, ld = 40000, 65536                                     # 2.6 G elements of fp16
+    rows = buf.view(torch.float16).as_strided((t, 3, 2, 64), (ld, 128, 64, 1))
+    rows.copy_(torch.randn(t, 3, 2, 64, generator=g, device="cuda"))
+    q, k, v = rows.unbind(1)
+    cu, cut = cu_of([39000, 900, 100])
+    out = ops.attention_packed(q, k, v, cut)
+    lo = 39000
+    attn_check(out[lo:], q[lo:], k[lo:], v[lo:], [0, 900, 1000])
+    flat = rows.as_strided((t, 384), (ld, 1))
+    norm_check([a[lo:] for a in ops.norm_residual(flat)], norm_all(flat[lo:], None, None, "none", "none", None, None, None, "rms", None, None))
+    pos, f = torch.arange(t, device="cuda")[:, None], torch.ones(32, device="cuda")
+    want = ops.rope_axes(q[lo:].contiguous(), None, pos[lo:], f, [32])
+    ops.rope_axes_(q, None, pos, f, [32])
+    assert torch.equal(q[lo:], want)
+
+
+@pytest.mark.gpu
+def test_grids_past_one_row():
+    """More workgroups than one row of the launch grid holds (2^18)."""
+    from sesa import ops
+    g = gen(22)
+    x = torch.randn(1_060_000, 16, generator=g, device="cuda").half()
+    q, s = ops.quantize_i8(x)
+    norm_check((x, q, s), (x.double(), x.double(), x.abs().amax(-1, keepdim=True).double(), x.abs().amax(-1, keepdim=True).double()), True)
+    x = torch.randn(262_200, 1032, generator=g, device="cuda", dtype=torch.float16)
+    y, n = ops.norm_residual(x)
+    at = torch.tensor([0, 262_143, 262_144, 262_199], device="cuda")
+    norm_check((y[at], n[at]), norm_all(x[at], None, None, "none", "none", None, None, None, "rms", None, None))
+    assert torch.equal(y, x)
+    del x, y, n
+    t = 300_000                                               # sequences of one token: each attends to itself alone
+    rows = torch.randn(t, 3, 1, 8, generator=g, device="cuda").half()
+    cut = torch.arange(t + 1, dtype=torch.int32, device="cuda")
+    assert torch.equal(ops.attention_packed(*rows.unbind(1), cut), rows[:, 2])
+    t = 67_200_000                                            # one pair a token: a thread each
+    x = torch.randn(t, 1, 2, generator=g, device="cuda", dtype=torch.float16)
+    pos = torch.arange(t, dtype=torch.int32, device="cuda")[:, None]
+    got = ops.rope_axes(x, None, pos, torch.full((1,), 0.001, device="cuda"), [1])
+    at = torch.tensor([0, 5, 67_108_863, 67_108_864, t - 1], device="cuda")
+    rope_check(got[at], x[at], pos[at], torch.full((1,), 0.001, device="cuda"), [1], "halves")
