@@ -3,6 +3,14 @@
 // One pass over the keys with a running maximum and sum (fp32).  S^T = K Q^T on v_mfma_*_32x32x16: a lane then holds
 // one query's scores, so the row statistics need a single exchange (the two lane halves), and the same registers,
 // rounded to the type, are the second operand of O^T += V^T P^T; V^T comes from LDS by transposing 16-bit reads.
+// Four waves of 32 queries share 64-key blocks of K and V in two LDS stages; blocks that every query of the tile sees run
+// without masks, the diagonal and the last one apart.  Two (head 128) to four (head 64) workgroups a CU, out of step with
+// each other, put one's softmax beside another's products: eight waves on one tile are slower (head 64 344 us where
+// four take 311, head 128 412 and 381), two waves read K and V from LDS for half the queries (501 at head 128).
+// Bound by the VALU about as much as by the matrix pipe: a 32 x 64 block is 32 exponentials and ~120 other operations
+// a lane (~1000 cycles) against 512 (head 64) or 1024 (head 128) cycles of products.  Measured: 12289 causal tokens,
+// 32 / 8 heads x 128, bf16 357-417 us by the sequences' lengths (0.93-1.05 PFLOP/s of its pairs); 2 x 801 tokens x 62
+// lanes, 8 heads x 64, fp16 259-268 us (0.63 PFLOP/s: 13 blocks a tile, one of them masked, 89 % of the query rows used).
 #include "sesa_tokens.h"
 
 namespace sesa {

@@ -2,6 +2,7 @@
 //
 // v_mfma_i32_16x16x64_i8 with the weights as the first operand: a lane's accumulators are then consecutive output
 // channels of one token.  The sums are exact 32-bit integers; scales, bias and activation are fp32, one rounding.
+// Measured: one token, 4096 -> 16384 (64 MB of weights) 17.1 us, 3.9 TB/s; 8192 tokens 482 us, 2.28 POP/s.
 //
 // Two kernels:
 //  * tile_kernel: BM tokens x BN channels per workgroup, K in 128-byte steps through a ring of LDS stages.
