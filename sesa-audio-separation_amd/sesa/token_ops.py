@@ -117,6 +117,21 @@ def _writable(t):
     return t.numel() == 0 or t.shape[-1] == 1 or t.stride(-1) == 1
 
 
+def _disjoint(ts, us, off):
+    """Whether two strided sets of elements share none; ts / us: (size, stride) from the widest stride down, u's first
+    element ``off`` behind t's.  False also where it is not plain to see."""
+    reach = [sum((n - 1) * s for n, s in d) + 1 for d in (ts, us)]
+    if off >= reach[0] or -off >= reach[1]:
+        return True
+    if not ts or not us or ts[0][1] != us[0][1]:
+        return False
+    row = ts[0][1]
+    if any(sum((n - 1) * s for n, s in d[1:]) + 1 > row for d in (ts, us)):
+        return False
+    at = off % row   # u's rows begin at..row behind, or row - at before, some row of t
+    return _disjoint(ts[1:], us[1:], at) and _disjoint(ts[1:], us[1:], at - row)
+
+
 def _apart(t, u):
     """Whether two tensors share no memory: by storage, by span, or as column ranges of the same rows."""
     if t.untyped_storage().data_ptr() != u.untyped_storage().data_ptr() or not t.numel() or not u.numel():
@@ -124,11 +139,10 @@ def _apart(t, u):
     a, b = t.data_ptr(), u.data_ptr()
     if a + _span(t) * t.element_size() <= b or b + _span(u) * u.element_size() <= a:
         return True
-    row = t.stride(0) * t.element_size()
-    if t.element_size() != u.element_size() or t.stride(0) != u.stride(0) or row <= 0:
+    if t.element_size() != u.element_size() or (b - a) % t.element_size():
         return False
-    at = (b - a) % row   # where u's columns begin, counted from t's in a row
-    return _span(t[0]) * t.element_size() <= at and at + _span(u[0]) * u.element_size() <= row
+    dims = [sorted(((n, s) for n, s in zip(x.shape, x.stride()) if n > 1), key=lambda d: -d[1]) for x in (t, u)]
+    return _disjoint(*dims, (b - a) // t.element_size())
 
 
 def _ptr(t):

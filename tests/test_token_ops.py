@@ -169,6 +169,33 @@ def test_memory_overlap_rules():
     assert not _writable(buf.as_strided((6, 2, 8), (8, 8, 1))) and not _writable(torch.zeros(1, 8).expand(4, 8))
 
 
+def test_memory_overlap_rules_against_sets():
+    """Never apart where two views share an element; apart for the layouts that projections write."""
+    from sesa.token_ops import _apart, _writable
+    import random
+    rng = random.Random(0)
+    buf = torch.zeros(4000)
+    found = 0
+    for _ in range(3000):
+        views = []
+        for _ in range(2):
+            shape = [rng.randint(1, 4) for _ in range(rng.randint(1, 4))]
+            base = rng.choice([1, 2, 3])
+            stride = sorted((base * rng.choice([1, 4, 8, 16, 24, 48, 96]) for _ in shape), reverse=rng.random() < 0.8)
+            views.append(buf.as_strided(shape, stride, rng.randint(0, 60)))
+        sets = [set((v.storage_offset() + sum(i * s for i, s in zip(ix, v.stride())) for ix in np.ndindex(*v.shape))) for v in views]
+        if _apart(*views):
+            found += 1
+            assert not sets[0] & sets[1], (views[0].shape, views[0].stride(), views[1].shape, views[1].stride())
+        for v, st in zip(views, sets):
+            assert not _writable(v) or len(st) == v.numel()
+    assert found > 100
+    rows = torch.zeros(5, 3, 18, 8)
+    q, k, v, o = rows.split([6, 3, 3, 6], 2)
+    assert all(_apart(a, o) and _apart(o, a) for a in (q, k, v)) and not _apart(rows[:, :, 5:7], q)
+    assert _apart(rows[..., :4], rows[..., 4:]) and not _apart(rows[..., :5], rows[..., 4:])
+
+
 # ---- GPU: linear_i8 -------------------------------------------------------------------------------------
 def linear_case(seed, m, k, n, bias=True, full=False):
     g = gen(seed)
@@ -850,3 +877,53 @@ def test_grids_past_one_row():
     got = ops.rope_axes(x, None, pos, torch.full((1,), 0.001, device="cuda"), [1])
     at = torch.tensor([0, 5, 67_108_863, 67_108_864, t - 1], device="cuda")
     rope_check(got[at], x[at], pos[at], torch.full((1,), 0.001, device="cuda"), [1], "halves")
+
+
+@pytest.mark.gpu
+def test_attention_packed_out_ranges_and_lane_groups():
+    """Lanes with grouped heads under a causal mask, and out as a column range of wider rows (the rest left alone)."""
+    from sesa import ops
+    cu, cut = cu_of([0, 130, 1, 60])
+    for d, dt in ((64, "bf16"), (128, "f16"), (40, "f16")):
+        q, k, v = qkv(31 + d, 191, 6, 3, d, dt, lanes=3)
+        gate = torch.randn(191, 3, 6, generator=gen(d), device="cuda").to(q.dtype)
+        want = ops.attention_packed(q, k, v, cut, gate=gate)
+        attn_check(want, q, k, v, cu, True, None, gate)
+        wide = torch.full((191, 3, 8, d + 5), 3.0, device="cuda", dtype=q.dtype)
+        ops.attention_packed(q, k, v, cut, gate=gate, out=wide[:, :, 1:7, 2:2 + d])
+        assert torch.equal(wide[:, :, 1:7, 2:2 + d], want)
+        wide[:, :, 1:7, 2:2 + d] = 3.0
+        assert bool((wide == 3).all())
+        rows = torch.cat([q, k, v, torch.zeros_like(q)], 2)   # out beside q, k, v in the same rows
+        qq, kk, vv, oo = rows.split([6, 3, 3, 6], 2)
+        ops.attention_packed(qq, kk, vv, cut, gate=gate, out=oo)
+        assert torch.equal(oo, want) and torch.equal(qq, q)
+
+
+@pytest.mark.gpu
+def test_token_ops_under_compile_and_modes():
+    """A traced call goes through the registered ops (fullgraph), an intercepting mode sees them."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+    from sesa import ops
+    blk = Block(128, 2, 1, 64, 5)
+    x, pos, cu, cut = block_inputs(6, 50, 128, [20, 30])
+    want = blk(x, pos, cut)
+
+    def f(x):
+        y, q, s = ops.norm_residual_i8(x, pre_weight=blk.norms[0])
+        z = ops.linear_i8(q, s, *blk.w["qkv"]).view(-1, 4, 64)
+        qq, kk = ops.rope_axes(z[:, :2], z[:, 2:3], pos, blk.freqs, blk.sections)
+        return y, ops.attention_packed(qq, kk, z[:, 3:], cut)
+    for a, b in zip(torch.compile(f, backend="aot_eager", fullgraph=True)(x), f(x)):
+        assert torch.equal(a, b)
+    seen = []
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+    with Watch():
+        got = blk(x, pos, cut)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for name in ("linear_i8", "norm_residual_i8", "norm_residual", "quantize_i8", "rope_axes_", "attention_packed"):
+        assert f"sesa.{name}.default" in seen, name
