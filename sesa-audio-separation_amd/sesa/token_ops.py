@@ -22,6 +22,7 @@ _ACT = {"none": 0, "gelu": 1, "tanh": 2, "relu": 3}
 _NORM = {"none": 0, "rms": 1, "layer": 2}
 _GATE = {"none": 0, "sigmoid": 1, "silu": 2, "tanh": 3}
 _LAYOUT = {"halves": 0, "pairs": 1}
+_INT4 = ctypes.c_int * 4
 
 _LIB = torch.library.Library("sesa", "FRAGMENT")
 
@@ -44,14 +45,22 @@ def _fail(op, msg):
 def _check(op, idx, names, *tensors):
     """Every tensor (None: absent) on device ``idx``, none of them waiting for a gradient."""
     grad = torch.is_grad_enabled()
-    for i, t in enumerate(tensors):
+    try:
+        for t in tensors:
+            if t is not None and (t.get_device() != idx or grad and t.requires_grad):
+                break
+        else:
+            return
+    except AttributeError:   # not a tensor
+        pass
+    for name, t in zip(names.split(), tensors):
         if t is None:
             continue
         if not isinstance(t, torch.Tensor) or t.get_device() != idx:
-            _fail(op, f"{names.split()[i]}: expected a HIP device tensor on cuda:{idx} (got {type(t).__name__} on "
+            _fail(op, f"{name}: expected a HIP device tensor on cuda:{idx} (got {type(t).__name__} on "
                       f"{getattr(t, 'device', None)}); the sesa path has no CPU fallback")
         if grad and t.requires_grad:
-            _fail(op, f"{names.split()[i]} requires a gradient and this operator has none (use torch.no_grad())")
+            _fail(op, f"{name} requires a gradient and this operator has none (use torch.no_grad())")
 
 
 def _device(op, t):
@@ -90,7 +99,7 @@ def _param(op, name, t, n):
     """An optional fp32 [n] parameter vector, contiguous."""
     if t is None:
         return None
-    if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != n:
+    if t.dtype is not torch.float32 or t.shape != (n,):
         _fail(op, f"{name}: expected float32 [{n}], got {t.dtype} {list(t.shape)}")
     return t if t.is_contiguous() else t.contiguous()
 
@@ -296,13 +305,14 @@ def _rope_call(op, xs, outs, positions, freqs, sections, layout):
     idx = _device(op, xs[0])
     _check(op, idx, "positions freqs q k", positions, freqs, *xs)
     x0 = xs[0]
+    shape, dtype = x0.shape, x0.dtype
     for x in xs:
-        if x.dim() != 3 or x.dtype not in _DTYPE or x.dtype != x0.dtype or x.shape[0] != x0.shape[0] or \
-                x.shape[2] != x0.shape[2]:
+        if x.dim() != 3 or dtype not in _DTYPE or x.dtype is not dtype or \
+                (x is not x0 and (x.shape[0] != shape[0] or x.shape[2] != shape[2])):
             _fail(op, f"expected [tokens, heads, head_dim] tensors of one type, token count and head_dim, got "
                       f"{[(str(t.dtype), list(t.shape)) for t in xs]}")
     if not 1 <= len(sections) <= 4 or positions.dim() != 2 or \
-            tuple(positions.shape) != (x0.shape[0], len(sections)) or \
+            positions.shape != (shape[0], len(sections)) or \
             positions.dtype not in (torch.int32, torch.int64):
         _fail(op, f"positions: expected int32 or int64 [{x0.shape[0]}, {len(sections)}] (1 to 4 axes), got "
                   f"{positions.dtype} {list(positions.shape)}")
@@ -310,12 +320,13 @@ def _rope_call(op, xs, outs, positions, freqs, sections, layout):
         _fail(op, f"layout {layout!r} (one of {', '.join(_LAYOUT)})")
     f = _param(op, "freqs", freqs, sum(sections))
     p = positions if len(sections) == 1 or positions.stride(1) == 1 else positions.contiguous()
-    a = N.SesaRopeArgs(x0.shape[0], x0.shape[2], _DTYPE[x0.dtype], _LAYOUT[layout], len(sections),
-                       (ctypes.c_int * 4)(*sections), p.data_ptr(), p.stride(0), p.dtype == torch.int64, f.data_ptr(),
-                       len(xs))
-    for i, (x, o) in enumerate(zip(xs, outs)):
-        a.t[i] = N.SesaRopeTensor(x.data_ptr(), x.stride(0), x.stride(1), o.data_ptr(), o.stride(0), o.stride(1),
-                                  x.shape[1])
+    a = N.SesaRopeArgs(x0.shape[0], x0.shape[2], _DTYPE[x0.dtype], _LAYOUT[layout], len(sections), _INT4(*sections),
+                       p.data_ptr(), p.stride(0), p.dtype is torch.int64, f.data_ptr(), len(xs))
+    for i, x in enumerate(xs):
+        o, r = outs[i], a.t[i]
+        r.x, r.out, r.heads = x.data_ptr(), o.data_ptr(), x.shape[1]
+        r.x_t, r.x_h, _ = x.stride()
+        r.o_t, r.o_h, _ = o.stride()
     _launch("rope_axes", idx, N.lib().sesa_rope_axes, ctypes.byref(a))
 
 

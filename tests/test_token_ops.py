@@ -927,3 +927,27 @@ def test_token_ops_under_compile_and_modes():
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     for name in ("linear_i8", "norm_residual_i8", "norm_residual", "quantize_i8", "rope_axes_", "attention_packed"):
         assert f"sesa.{name}.default" in seen, name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [40, 64, 96, 128])
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+def test_attention_packed_non_finite_values_of_long_sequences(d, dt):
+    """One infinite value row early in a sequence of several tiles: the rows before it stay finite, the others get it, in
+    its own tile (a masked block) and in later ones (whole blocks)."""
+    from sesa import ops
+    cu, cut = cu_of([300, 80])
+    q, k, v = (x.clone() for x in qkv(40 + d, 380, 4, 2, d, dt))
+    clean = ops.attention_packed(q, k, v, cut)
+    v[5, :, 3] = math.inf
+    got = ops.attention_packed(q, k, v, cut)
+    attn_check(got[:5], q[:5], k[:5], v[:5], [0, 5])
+    assert torch.equal(got[300:], clean[300:])
+    tail = got[5:300].float()
+    assert bool((tail[..., 3] == math.inf).all()) and bool(torch.isfinite(torch.cat([tail[..., :3], tail[..., 4:]], -1)).all())
+    v[5, :, 3] = 0.5   # (finite again: the other columns of those rows were what they are now)
+    ref = ops.attention_packed(q, k, v, cut)
+    keep = [c for c in range(d) if c != 3]
+    u = HALF[q.dtype]
+    assert bool(((got[:300][..., keep] - ref[:300][..., keep]).double().abs() <=
+                 3 * u * (ref[:300][..., keep].double().abs() + float(v.abs().max()))).all())
