@@ -73,26 +73,28 @@ def _device(op, t):
 
 def _launch(op, idx, entry, *args):
     """``entry(*args, stream)`` with device ``idx`` current, on its current stream."""
-    if torch.cuda.current_device() == idx:
-        rc = entry(*args, torch._C._cuda_getCurrentRawStream(idx))
+    if _current_device() == idx:
+        rc = entry(*args, _current_stream(idx))
     else:
         with torch.cuda.device(idx):
-            rc = entry(*args, torch._C._cuda_getCurrentRawStream(idx))
+            rc = entry(*args, _current_stream(idx))
     if rc:
         N.check(rc, f"sesa_{op}")
 
 
+_Tensor = torch.Tensor
+_compiling = torch.compiler.is_compiling
 _modes = getattr(torch._C, "_len_torch_dispatch_stack", lambda: 1)
+_current_device = torch.cuda.current_device
+_current_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _eager(op, t):
     """Whether a call can go straight to its device kernel: a plain device tensor, nothing tracing or intercepting the
     ops.  Saves the dispatcher's share of the host's time (3 to 4 us a call: a one-token call takes 5 to 8)."""
-    if type(t) is torch.Tensor:
+    if not isinstance(t, _Tensor) or not t.is_cuda:
         _device(op, t)
-        return not torch.compiler.is_compiling() and not _modes()
-    _device(op, t)
-    return False
+    return type(t) is _Tensor and not _compiling() and not _modes()
 
 
 def _param(op, name, t, n):
@@ -239,14 +241,23 @@ def _norm_call(op, x, residual, gate, gate_act, post, post_weight, post_bias, sc
     y = torch.empty_like(x if residual is None else residual, memory_format=torch.contiguous_format)
     n = torch.empty_like(x, dtype=torch.int8 if i8 else None, memory_format=torch.contiguous_format)
     qs = x.new_empty(x.shape[:-1], dtype=torch.float32) if i8 else None
-    pw, pb = _param(op, "post_weight", post_weight, d), _param(op, "post_bias", post_bias, d)
-    nw, nb = _param(op, "pre_weight", pre_weight, d), _param(op, "pre_bias", pre_bias, d)
-    sc = _param(op, "scale", scale, d)
-    a = N.SesaNormArgs(
-        xr.shape[0], d, _DTYPE[x.dtype], _DTYPE[rt], xr.data_ptr(), xr.stride(0), _ptr(rr),
-        0 if rr is None else rr.stride(0), _ptr(gr), 0 if gr is None else gr.stride(0), per, _GATE[gate_act],
-        _NORM[post], _ptr(pw), _ptr(pb), _ptr(sc), _NORM[pre], _ptr(nw), _ptr(nb), eps, y.data_ptr(), d,
-        None if i8 else n.data_ptr(), d, n.data_ptr() if i8 else None, d, _ptr(qs))
+    a = N.SesaNormArgs(xr.shape[0], d, _DTYPE[x.dtype], _DTYPE[rt], xr.data_ptr(), xr.stride(0))
+    if rr is not None:
+        a.residual, a.r_ld = rr.data_ptr(), rr.stride(0)
+    if gr is not None:
+        a.gate, a.gate_ld, a.rows_per_gate, a.gate_act = gr.data_ptr(), gr.stride(0), per, _GATE[gate_act]
+    a.post, a.pre, a.eps = _NORM[post], _NORM[pre], eps
+    kept = []   # copies live until the launch
+    for name, t in (("post_weight", post_weight), ("post_bias", post_bias), ("scale", scale), ("pre_weight", pre_weight),
+                    ("pre_bias", pre_bias)):
+        if t is not None:
+            kept.append(_param(op, name, t, d))
+            setattr(a, name, kept[-1].data_ptr())
+    a.y, a.y_ld = y.data_ptr(), d
+    if i8:
+        a.q, a.q_ld, a.q_scale = n.data_ptr(), d, qs.data_ptr()
+    else:
+        a.n, a.n_ld = n.data_ptr(), d
     _launch("norm_residual", idx, N.lib().sesa_norm_residual, ctypes.byref(a))
     return (y, n, qs) if i8 else (y, n)
 
