@@ -59,11 +59,13 @@ __device__ __forceinline__ bool find_tile(const sesa_attn_args& a, int slot, int
   return q >= b && q < e;
 }
 
-// DMA: rows of exactly D elements at 16-byte addresses, K and V go to LDS by global_load_lds_dwordx4 (no registers, no
-// LDS stores; keys behind the sequence repeat its last one).  Otherwise through registers, zeros behind the sequence
-// and behind head_dim.
-template <class T, int D, int NW, bool DMA>
-__global__ void __launch_bounds__(NW * 64, D == 64 ? (DMA ? 4 : 3) : 2) attn_packed_kernel(sesa_attn_args a, int n_slots, int n_blocks_all) {
+// kDma: rows of exactly D elements at 16-byte addresses, K and V go to LDS by global_load_lds_dwordx4 (no registers, no
+// LDS stores; keys behind the sequence repeat its last one).  kDmaPart: the same for fewer elements, those behind head_dim
+// zeroed once and their lanes kept out of the loads.  kRegisters: zeros behind the sequence and behind head_dim.
+enum { kRegisters, kDma, kDmaPart };
+template <class T, int D, int NW, int LOADS>
+__global__ void __launch_bounds__(NW * 64, D == 64 ? (LOADS != kRegisters ? 4 : 3) : 2) attn_packed_kernel(sesa_attn_args a, int n_slots, int n_blocks_all) {
+  constexpr bool DMA = LOADS != kRegisters, PART = LOADS == kDmaPart;
   constexpr int BQ = NW * 32, NTH = NW * 64, ROW = D * 2, IMG = kKeys * ROW, CH = D / 8, IT = kKeys * CH / NTH;
   constexpr float kLog2e = 1.4426950408889634f;
   __shared__ __attribute__((aligned(16))) char smem[4 * IMG];   // [stage][K, V], rows of D elements
@@ -121,10 +123,13 @@ __global__ void __launch_bounds__(NW * 64, D == 64 ? (DMA ? 4 : 3) : 2) attn_pac
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
   constexpr int PCS = IMG / 1024 / NW, RPP = 1024 / ROW;   // pieces per wave and image, rows per piece
   uint32_t koff[DMA ? PCS : 1], voff[DMA ? PCS : 1];
+  uint32_t inside = 0;   // bit i: this lane's chunk of piece i lies inside head_dim (kDmaPart)
+  auto lds_base = [](uint32_t v) { return PART ? (uint32_t)__builtin_amdgcn_readfirstlane(v) : v; };   // m0 inside a branch
   auto offsets = [&](int n) {   // n: keys of the block that exist
 #pragma unroll
     for (int i = 0; i < PCS; ++i) {
       const int row = (wave + NW * i) * RPP + lane / CH, ch = (lane % CH) ^ key_of(row), r = min(row, n - 1);
+      if constexpr (PART) inside |= (uint32_t)(ch * 8 < hd) << i;
       koff[i] = (uint32_t)(r * (int)a.k_t + ch * 8) * 2u;
       voff[i] = (uint32_t)(r * (int)a.v_t + ch * 8) * 2u;
     }
@@ -137,9 +142,11 @@ __global__ void __launch_bounds__(NW * 64, D == 64 ? (DMA ? 4 : 3) : 2) attn_pac
       const char* kb0 = reinterpret_cast<const char*>(kp + p0 * a.k_t);
       const char* vb0 = reinterpret_cast<const char*>(vp + p0 * a.v_t);
 #pragma unroll
-      for (int i = 0; i < PCS; ++i) dma16_asm(kb0, koff[i], lds0 + stage + (wave + NW * i) * 1024);
+      for (int i = 0; i < PCS; ++i)
+        if (!PART || (inside >> i & 1)) dma16_asm(kb0, koff[i], lds_base(lds0 + stage + (wave + NW * i) * 1024));
 #pragma unroll
-      for (int i = 0; i < PCS; ++i) dma16_asm(vb0, voff[i], lds0 + stage + IMG + (wave + NW * i) * 1024);
+      for (int i = 0; i < PCS; ++i)
+        if (!PART || (inside >> i & 1)) dma16_asm(vb0, voff[i], lds_base(lds0 + stage + IMG + (wave + NW * i) * 1024));
     } else {
 #pragma unroll
       for (int i = 0; i < IT; ++i) {
@@ -274,7 +281,13 @@ __global__ void __launch_bounds__(NW * 64, D == 64 ? (DMA ? 4 : 3) : 2) attn_pac
     if (kb + 1 < n_blocks) store_block(next);
   };
 
-  if constexpr (DMA) offsets(min(kKeys, end - start));
+  if constexpr (DMA) {
+    offsets(min(kKeys, end - start));
+    if constexpr (PART) {
+      for (int e = tid * 16; e < 4 * IMG; e += NTH * 16) *reinterpret_cast<u32x4*>(smem + e) = u32x4{0u, 0u, 0u, 0u};
+      sesa_sync();
+    }
+  }
   load_block(0, 0);
   store_block(0);
   __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0), where the compiler sees it: no wait for Q inside the loop
@@ -346,20 +359,22 @@ int launch_attn(const sesa_attn_args& a, hipStream_t st) {
   const int64_t n_slots = a.tokens / (NW * 32) + a.n_seq + 2;
   const int64_t blocks = n_slots * a.heads * a.lanes;
   SESA_REQUIRE(blocks < (1ll << 31), SESA_ERR_INVALID, "attention_packed: too many tokens x heads x lanes");
-  // 16-byte rows of a whole tile width, and a block's byte offsets in 32 bits
-  auto dma = [&](int D) {
-    const int64_t strides = a.k_t | a.k_l | a.k_h | a.v_t | a.v_l | a.v_h;
-    return a.head_dim == D && strides % 8 == 0 && ((uintptr_t)a.k | (uintptr_t)a.v) % 16 == 0 && a.k_t >= 0 &&
-           a.v_t >= 0 && a.k_t < (1 << 23) && a.v_t < (1 << 23);
-  };
+  // 16-byte rows, and a block's byte offsets in 32 bits.  Rows of the whole tile width have a kernel of their own (12289
+  // causal tokens, 32 / 8 heads of 128, bf16: 385 us, 402 with the part rows' masks); part rows at 96 of 128 elements: 488
+  // us, 582 through registers.
+  const int64_t strides = a.k_t | a.k_l | a.k_h | a.v_t | a.v_l | a.v_h;
+  const bool dma = strides % 8 == 0 && ((uintptr_t)a.k | (uintptr_t)a.v) % 16 == 0 && a.k_t >= 0 && a.v_t >= 0 &&
+                   a.k_t < (1 << 23) && a.v_t < (1 << 23);
   const dim3 grid = long_grid(blocks), block(NW * 64);
   const int nb = (int)blocks;
   if (a.head_dim <= 64) {
-    if (dma(64)) hipLaunchKernelGGL((attn_packed_kernel<T, 64, NW, true>), grid, block, 0, st, a, (int)n_slots, nb);
-    else hipLaunchKernelGGL((attn_packed_kernel<T, 64, NW, false>), grid, block, 0, st, a, (int)n_slots, nb);
+    if (!dma) hipLaunchKernelGGL((attn_packed_kernel<T, 64, NW, kRegisters>), grid, block, 0, st, a, (int)n_slots, nb);
+    else if (a.head_dim == 64) hipLaunchKernelGGL((attn_packed_kernel<T, 64, NW, kDma>), grid, block, 0, st, a, (int)n_slots, nb);
+    else hipLaunchKernelGGL((attn_packed_kernel<T, 64, NW, kDmaPart>), grid, block, 0, st, a, (int)n_slots, nb);
   } else {
-    if (dma(128)) hipLaunchKernelGGL((attn_packed_kernel<T, 128, NW, true>), grid, block, 0, st, a, (int)n_slots, nb);
-    else hipLaunchKernelGGL((attn_packed_kernel<T, 128, NW, false>), grid, block, 0, st, a, (int)n_slots, nb);
+    if (!dma) hipLaunchKernelGGL((attn_packed_kernel<T, 128, NW, kRegisters>), grid, block, 0, st, a, (int)n_slots, nb);
+    else if (a.head_dim == 128) hipLaunchKernelGGL((attn_packed_kernel<T, 128, NW, kDma>), grid, block, 0, st, a, (int)n_slots, nb);
+    else hipLaunchKernelGGL((attn_packed_kernel<T, 128, NW, kDmaPart>), grid, block, 0, st, a, (int)n_slots, nb);
   }
   SESA_CHECK_LAUNCH();
   return SESA_OK;

@@ -673,6 +673,24 @@ def test_attention_packed_non_finite(d, dt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("d", [8, 40, 56, 72, 96, 120])
+def test_attention_packed_part_rows(d):
+    """Rows narrower than the tile: copied at 16-byte addresses and through registers alike, and nothing of the element
+    behind a row (another head's NaN and infinity) reaches it."""
+    from sesa import ops
+    cu, cut = cu_of([300, 0, 65, 129])
+    for causal in (True, False):
+        q, k, v = qkv(d + 7, cu[-1], 6, 3, d, "bf16")
+        got = ops.attention_packed(q, k, v, cut, causal=causal)
+        attn_check(got, q, k, v, cu, causal)
+        odd = [torch.nn.functional.pad(x, (1, 2))[..., 1:d + 1] for x in (q, k, v)]
+        assert torch.equal(ops.attention_packed(*odd, cut, causal=causal), got)
+        k2, v2 = k.clone(), v.clone()
+        k2[:, 2], v2[:, 2], k2[:, 0], v2[:, 0] = math.nan, math.inf, math.inf, math.nan
+        assert torch.equal(ops.attention_packed(q, k2, v2, cut, causal=causal)[:, 2:4], got[:, 2:4])
+
+
+@pytest.mark.gpu
 def test_attention_packed_large_scores():
     """Scores far apart (the running maximum moves by more than the lazy step, P under- and overflows without it)."""
     from sesa import ops
