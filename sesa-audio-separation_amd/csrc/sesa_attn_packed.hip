@@ -109,8 +109,14 @@ __global__ void __launch_bounds__(NW * 64, D == 64 ? (LOADS != kRegisters ? 4 : 
   for (int db = 0; db < D / 32; ++db)
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[db][r] = 0.f;
-  float m_run = -INFINITY, l_run = 0.f;   // running maximum (of the raw scores) and sum
+  // Running reference r_run = a largest score so far times c, rounded to fp32, and the running sum.  Every probability is
+  // exp2(s c - r_run) with the product unrounded: the reference's own rounding is in all of them alike and cancels (a
+  // product rounded anew for each use would not: 6e-2 of a block's weight at scores of 1e6).  From kFar on that rounding
+  // may reach a factor of 2^0.5 and, further out, the range of P, so such rows are done over below.
+  float r_run = -INFINITY, l_run = 0.f;
   const float c = a.scale * kLog2e;
+  constexpr float kFar = 4194304.f;   // 2^22: fp32 steps of 2^-1
+  bool far = false;
 
   // 16-byte chunk c of row r lies at c ^ key(r).  A K fragment read takes one chunk of 8 rows at a time, a transposing V
   // read four chunks of 4 rows: both sets fall into different banks (256 B of them: two rows of 64 elements, one of 128).
@@ -236,23 +242,25 @@ __global__ void __launch_bounds__(NW * 64, D == 64 ? (LOADS != kRegisters ? 4 : 
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[rb][r]);
     top = max_halves(top);
-    // The running maximum moves only when a block exceeds it by more than 2^8 in the exponential (P stays <= 256, in
+    // The reference moves only when a block exceeds it by more than 2^8 in the exponential (P stays <= 256 or so, in
     // range for fp16), so most blocks leave O alone.  Both halves of a query hold the same values, so they agree.
-    if ((top - m_run) * c > 8.f) {
-      const float alpha = __builtin_amdgcn_exp2f((m_run - top) * c);   // (the first time: 0)
+    if (fmaf(top, c, -r_run) > 8.f) {
+      const float r = top * c;
+      const float alpha = __builtin_amdgcn_exp2f(r_run - r);   // (the first time: 0)
+      far = far || (fabsf(top) < INFINITY && !(fabsf(r) <= kFar));
       l_run *= alpha;
 #pragma unroll
       for (int db = 0; db < D / 32; ++db)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
-      m_run = top;
+      r_run = r;
     }
-    const float mc = m_run == -INFINITY ? 0.f : m_run * c;   // (no finite score so far: every P is exp(-inf) = 0)
+    const float rc = r_run == -INFINITY ? 0.f : r_run;   // (no finite score so far: every P is exp(-inf) = 0)
 #pragma unroll
     for (int rb = 0; rb < 2; ++rb)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(s[rb][r], c, -mc));
+        const float p = __builtin_amdgcn_exp2f(fmaf(s[rb][r], c, -rc));
         s[rb][r] = p;
         l_run += p;   // this half's keys; the halves join at the end
       }
@@ -296,11 +304,12 @@ __global__ void __launch_bounds__(NW * 64, D == 64 ? (LOADS != kRegisters ? 4 : 
   for (; kb < n_blocks; ++kb) step(kb, std::true_type{});
   l_run += __shfl_xor(l_run, 32);
 
-  if (__ballot((bad & 0x80008000u) != 0)) {
+  if (__ballot(far || (bad & 0x80008000u) != 0)) {
     // Rare: the wave's queries key by key, each only with the keys it sees, from global memory and without matrix
     // instructions (no barrier: the waves of the tile may differ).  A lane half has its half of q's and o's elements.
+    // The maximum is taken off before the scaling: exactly 0 at the largest score, whatever its size.
     const int64_t lim = min((int64_t)(end - 1), a.causal ? q_pos : (int64_t)(end - 1));
-    m_run = -INFINITY;
+    float m_run = -INFINITY;
     l_run = 0.f;
 #pragma unroll
     for (int db = 0; db < D / 32; ++db)
@@ -324,8 +333,8 @@ __global__ void __launch_bounds__(NW * 64, D == 64 ? (LOADS != kRegisters ? 4 : 
       dot += __shfl_xor(dot, 32);
       if (j > lim) continue;
       const float top = fmaxf(m_run, dot);
-      const float base = top == -INFINITY ? 0.f : top * c;
-      const float alpha = __builtin_amdgcn_exp2f(fmaf(m_run, c, -base)), p = __builtin_amdgcn_exp2f(fmaf(dot, c, -base));
+      const float base = top == -INFINITY ? 0.f : top;
+      const float alpha = __builtin_amdgcn_exp2f((m_run - base) * c), p = __builtin_amdgcn_exp2f((dot - base) * c);
       m_run = top;
       l_run = fmaf(l_run, alpha, p);
 #pragma unroll
