@@ -206,7 +206,6 @@ __global__ void __launch_bounds__(NW * 64, D == 64 ? (LOADS != kRegisters ? 4 : 
   // blocks all of whose keys every query of the tile sees
   const int n_whole = (min(end, a.causal ? q0 + 1 : end) - start) / kKeys;
 
-  uint32_t bad = 0;   // bits 15 and 31: a non-finite v in a masked block
   auto step = [&](int kb, auto masked) {
     constexpr bool MASKED = decltype(masked)::value;
     const int cur = (kb & 1) * 2 * IMG, next = ((kb + 1) & 1) * 2 * IMG;
@@ -273,16 +272,6 @@ __global__ void __launch_bounds__(NW * 64, D == 64 ? (LOADS != kRegisters ? 4 : 
       u32x4 vf[D / 32];
 #pragma unroll
       for (int db = 0; db < D / 32; ++db) vf[db] = vt(cur, ks, db);
-      if constexpr (MASKED) {
-        // A masked block multiplies probabilities of 0 with the keys its rows do not see: harmless for finite v, but
-        // 0 * inf is NaN.  So look for non-finite v (exponent all ones); a wave that meets any starts over below.
-        constexpr uint32_t kExp = std::is_same<T, f16>::value ? 0x7c007c00u : 0x7f807f80u;
-        constexpr uint32_t kOne = std::is_same<T, f16>::value ? 0x04000400u : 0x00800080u;
-#pragma unroll
-        for (int db = 0; db < D / 32; ++db)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) bad |= (vf[db][q] & kExp) + kOne;
-      }
 #pragma unroll
       for (int db = 0; db < D / 32; ++db) o[db] = mfma16<T>(vf[db], pf, o[db]);
     }
@@ -304,17 +293,34 @@ __global__ void __launch_bounds__(NW * 64, D == 64 ? (LOADS != kRegisters ? 4 : 
   for (; kb < n_blocks; ++kb) step(kb, std::true_type{});
   l_run += __shfl_xor(l_run, 32);
 
-  if (__ballot(far || (bad & 0x80008000u) != 0)) {
-    // Rare: the wave's queries key by key, each only with the keys it sees, from global memory and without matrix
-    // instructions (no barrier: the waves of the tile may differ).  A lane half has its half of q's and o's elements.
-    // The maximum is taken off before the scaling: exactly 0 at the largest score, whatever its size.
+  // Rows to do over: `far`, and NaN in o under finite probabilities.  A probability of 0 -- a key that the row does not see,
+  // or one too small for the type -- times an infinite or NaN v is NaN, and so is an infinity times a rescaling by 0.
+  // (NaN scores make the sum NaN as well: that row is NaN by the formula.)  Nothing to look for inside the loop.
+  bool over = false;
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) over = over || o[db][r] != o[db][r];
+  over = far || (over && l_run == l_run);
+  const uint64_t redo = __ballot(over);
+  if (redo) {
+    // Rare, and bound by the latency of one key after the other, 2.4 us (12289 causal tokens, 32 / 8 heads x 128, bf16: 0.4
+    // ms; NaN in the last token 30 ms, scores of 1e9 in every row 69 ms): those rows key by key, each only with the keys it sees, from global memory and without matrix instructions
+    // (no barrier: the waves of the tile may differ); the wave's other rows keep what they have.  A lane half has its half
+    // of q's and o's elements.  The maximum is taken off before the scaling: exactly 0 at the largest score, whatever its
+    // size.  A finite score never weighs less than kLeast, nor does a rescaling: too little to move a finite sum, and an
+    // infinite v stays what it is.
+    constexpr float kLeast = 1.17549435e-38f;   // 2^-126
+    const bool mine = ((uint32_t)(redo >> 32) | (uint32_t)redo) >> l32 & 1;
     const int64_t lim = min((int64_t)(end - 1), a.causal ? q_pos : (int64_t)(end - 1));
     float m_run = -INFINITY;
-    l_run = 0.f;
+    if (mine) {
+      l_run = 0.f;
 #pragma unroll
-    for (int db = 0; db < D / 32; ++db)
+      for (int db = 0; db < D / 32; ++db)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) o[db][r] = 0.f;
+        for (int r = 0; r < 16; ++r) o[db][r] = 0.f;
+    }
 #pragma unroll 1
     for (int64_t j = start; j < last; ++j) {
       const T* kj = kp + j * a.k_t;
@@ -331,10 +337,12 @@ __global__ void __launch_bounds__(NW * 64, D == 64 ? (LOADS != kRegisters ? 4 : 
         }
       }
       dot += __shfl_xor(dot, 32);
-      if (j > lim) continue;
+      if (j > lim || !mine) continue;
       const float top = fmaxf(m_run, dot);
       const float base = top == -INFINITY ? 0.f : top;
-      const float alpha = __builtin_amdgcn_exp2f((m_run - base) * c), p = __builtin_amdgcn_exp2f((dot - base) * c);
+      const float alpha = fmaxf(__builtin_amdgcn_exp2f((m_run - base) * c), kLeast);
+      float p = __builtin_amdgcn_exp2f((dot - base) * c);
+      if (p < kLeast && dot > -INFINITY) p = kLeast;
       m_run = top;
       l_run = fmaf(l_run, alpha, p);
 #pragma unroll

@@ -94,3 +94,56 @@ def test_attention_random_far_scores(d, dt, val):
             want = v[a:b, h][at[:, 0]]
             assert bool(((got[a:b, h] - want).double().abs() <= 2 * HALF[v.dtype] * (want.double().abs() + 0.01))[sure].all())
     assert clear > 377
+
+
+# ---- attention_packed: infinite and NaN values ---------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("gap", [10.0, 14.0, 60.0, 95.0, 400.0])
+@pytest.mark.parametrize("d,dt", [(64, "f16"), (128, "f16"), (40, "f16"), (64, "bf16"), (128, "bf16")])
+def test_attention_infinite_values_at_small_probabilities(d, dt, gap):
+    """A visible infinity counts however small its probability is (e^-gap of the largest), wherever its key lies in its
+    block, also when the maximum moves behind it; a key that a row does not see counts for nothing."""
+    from sesa import ops
+    cu, cut = cu_of([300, 140])
+    g = gen(d)
+    q = torch.zeros(440, 2, d, device="cuda", dtype=DT[dt])
+    k = torch.zeros_like(q)
+    q[..., 0] = 1.0
+    level = torch.rand(440, generator=g, device="cuda")
+    level[[5, 70, 299, 303]] -= gap            # in whole and in masked blocks, at the ends of the sequences
+    level[200] += gap / 2                       # the maximum moves far behind the first infinities
+    k[..., 0] = level[:, None].to(DT[dt])
+    v = torch.randn(440, 2, d, generator=g, device="cuda").to(DT[dt])
+    clean = {c: ops.attention_packed(q, k, v, cut, causal=c, scale=1.0) for c in (True, False)}
+    v[5, :, 3], v[70, :, 4], v[299, :, 5], v[303, :, 6] = math.inf, -math.inf, math.inf, -math.inf
+    for causal in (True, False):
+        got = ops.attention_packed(q, k, v, cut, causal=causal, scale=1.0)
+        want = clean[causal].double()
+        for key, end, col, val in ((5, 300, 3, math.inf), (70, 300, 4, -math.inf), (299, 300, 5, math.inf), (303, 440, 6, -math.inf)):
+            want[key if causal else 300 * (key >= 300):end, :, col] = val
+        # finite columns: two results of the same rows, each a rounding of P and of itself off
+        x = torch.where(torch.isfinite(v), v, 0).double().abs().amax()
+        close(got, want, 4 * HALF[v.dtype] * x)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,dt", [(64, "f16"), (128, "bf16"), (96, "f16")])
+def test_attention_rows_beside_non_finite_ones_keep_their_bits(d, dt):
+    """Of the rows of one tile, those that see no NaN and whose masked keys hold none are what they are without it."""
+    from sesa import ops
+    cu, cut = cu_of([400])
+    g = gen(d)
+    q, k, v = (torch.randn(400, 2, d, generator=g, device="cuda").to(DT[dt]) for _ in range(3))
+    clean = ops.attention_packed(q, k, v, cut)
+    v[200, 0, 1] = math.nan
+    got = ops.attention_packed(q, k, v, cut)
+    assert torch.equal(got[:, 1], clean[:, 1]) and torch.equal(got[:128], clean[:128])   # another head, earlier blocks
+    assert bool(torch.isnan(got[200:, 0, 1]).all()) and int(torch.isnan(got).sum()) == 200
+    off = (got[:, 0].double() - clean[:, 0].double()).abs()
+    off[:, 1] = torch.where(torch.arange(400, device="cuda") < 200, off[:, 1], 0)
+    assert float(off.max()) <= 4 * HALF[v.dtype] * float(torch.nan_to_num(v).abs().max())
+    q[300, 0] = math.nan                                                  # a NaN query: its row and no other
+    got2 = ops.attention_packed(q, k, v, cut)
+    assert bool(torch.isnan(got2[300, 0]).all())
+    keep = torch.arange(400, device="cuda") != 300
+    assert torch.equal(torch.nan_to_num(got2[keep]), torch.nan_to_num(got[keep]))
