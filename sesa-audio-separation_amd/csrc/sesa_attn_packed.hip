@@ -109,10 +109,13 @@ __global__ void __launch_bounds__(NW * 64, D == 64 ? (LOADS != kRegisters ? 4 : 
   for (int db = 0; db < D / 32; ++db)
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[db][r] = 0.f;
-  // Running reference r_run = a largest score so far times c, rounded to fp32, and the running sum.  Every probability is
+  // Running reference r_run = a largest score so far times c (less kLift), rounded to fp32, and the running sum.  Every probability is
   // exp2(s c - r_run) with the product unrounded: the reference's own rounding is in all of them alike and cancels (a
   // product rounded anew for each use would not: 6e-2 of a block's weight at scores of 1e6).  From kFar on that rounding
   // may reach a factor of 2^0.5 and, further out, the range of P, so such rows are done over below.
+  // kLift: fp16 takes P 2^7 higher, so that it is normal down to 2^-21 of the largest where plain P ends at 2^-14 (below,
+  // a step is 2^-24: 100000 keys at 1.5 steps each lost a third of their weight).
+  constexpr float kLift = std::is_same<T, f16>::value ? 7.f : 0.f;
   float r_run = -INFINITY, l_run = 0.f;
   const float c = a.scale * kLog2e;
   constexpr float kFar = 4194304.f;   // 2^22: fp32 steps of 2^-1
@@ -241,10 +244,10 @@ __global__ void __launch_bounds__(NW * 64, D == 64 ? (LOADS != kRegisters ? 4 : 
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[rb][r]);
     top = max_halves(top);
-    // The reference moves only when a block exceeds it by more than 2^8 in the exponential (P stays <= 256 or so, in
+    // The reference moves only when a block exceeds it by more than 2^8 in the exponential (P stays below 2^(8.5 + kLift), in
     // range for fp16), so most blocks leave O alone.  Both halves of a query hold the same values, so they agree.
-    if (fmaf(top, c, -r_run) > 8.f) {
-      const float r = top * c;
+    if (fmaf(top, c, -r_run) > 8.f + kLift) {
+      const float r = fmaf(top, c, -kLift);
       const float alpha = __builtin_amdgcn_exp2f(r_run - r);   // (the first time: 0)
       far = far || (fabsf(top) < INFINITY && !(fabsf(r) <= kFar));
       l_run *= alpha;
@@ -255,14 +258,16 @@ __global__ void __launch_bounds__(NW * 64, D == 64 ? (LOADS != kRegisters ? 4 : 
       r_run = r;
     }
     const float rc = r_run == -INFINITY ? 0.f : r_run;   // (no finite score so far: every P is exp(-inf) = 0)
+    float sum[2] = {0.f, 0.f};   // a block's own first: small ones would be lost one by one against a large l_run
 #pragma unroll
     for (int rb = 0; rb < 2; ++rb)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const float p = __builtin_amdgcn_exp2f(fmaf(s[rb][r], c, -rc));
         s[rb][r] = p;
-        l_run += p;   // this half's keys; the halves join at the end
+        sum[rb] += p;
       }
+    l_run += sum[0] + sum[1];   // this half's keys; the halves join at the end
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
       f32x16& sv = s[ks >> 1];
@@ -305,11 +310,11 @@ __global__ void __launch_bounds__(NW * 64, D == 64 ? (LOADS != kRegisters ? 4 : 
   const uint64_t redo = __ballot(over);
   if (redo) {
     // Rare, and bound by the latency of one key after the other, 2.4 us (12289 causal tokens, 32 / 8 heads x 128, bf16: 0.4
-    // ms; NaN in the last token 30 ms, scores of 1e9 in every row 69 ms): those rows key by key, each only with the keys it sees, from global memory and without matrix instructions
-    // (no barrier: the waves of the tile may differ); the wave's other rows keep what they have.  A lane half has its half
-    // of q's and o's elements.  The maximum is taken off before the scaling: exactly 0 at the largest score, whatever its
-    // size.  A finite score never weighs less than kLeast, nor does a rescaling: too little to move a finite sum, and an
-    // infinite v stays what it is.
+    // ms; NaN in the last token 30 ms, scores of 1e9 in every row 69 ms): those rows key by key, each only with the keys
+    // it sees, from global memory and without matrix instructions (no barrier: the waves of the tile may differ); the
+    // wave's other rows keep what they have.  A lane half has its half of q's and o's elements.  The maximum is taken off
+    // before the scaling: exactly 0 at the largest score, whatever its size.  A finite score never weighs less than
+    // kLeast, nor does a rescaling: too little to move a finite sum, and an infinite v stays what it is.
     constexpr float kLeast = 1.17549435e-38f;   // 2^-126
     const bool mine = ((uint32_t)(redo >> 32) | (uint32_t)redo) >> l32 & 1;
     const int64_t lim = min((int64_t)(end - 1), a.causal ? q_pos : (int64_t)(end - 1));

@@ -147,3 +147,25 @@ def test_attention_rows_beside_non_finite_ones_keep_their_bits(d, dt):
     assert bool(torch.isnan(got2[300, 0]).all())
     keep = torch.arange(400, device="cuda") != 300
     assert torch.equal(torch.nan_to_num(got2[keep]), torch.nan_to_num(got[keep]))
+
+
+# ---- attention_packed: many small probabilities --------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,dt,n", [(64, "f16", 100_000), (128, "f16", 60_001), (64, "bf16", 100_000), (48, "f16", 100_000)])
+def test_attention_one_large_score_over_many_small_ones(d, dt, n):
+    """One key takes most of a row and a long sequence of small probabilities the rest: about 2^-23.4 each, which fp16 (and
+    an fp32 sum that adds them one by one) would round by a third."""
+    from sesa import ops
+    q = torch.zeros(n, 1, d, device="cuda", dtype=DT[dt])
+    k = torch.zeros_like(q)
+    q[..., 0], k[3, 0, 0] = 1.0, 16.234375
+    gap = float(k[3, 0, 0])
+    v = torch.ones_like(q)
+    v[3] = -1.0
+    m = (n - 1) * math.exp(-gap)
+    ref = (m - 1) / (m + 1)
+    got = ops.attention_packed(q, k, v, causal=False, scale=1.0).double()
+    u = HALF[DT[dt]]
+    # small weights rounded to the type, exp2, n / 64 block sums and n / 16 products added in fp32, the result's rounding
+    tol = m * (u + 2.0 ** -20) + (n / 64 + n / 16) * 2.0 ** -24 + u * 1.01
+    assert float((got - ref).abs().max()) <= tol, (float((got - ref).abs().max()), tol, ref)
