@@ -329,7 +329,7 @@ int sesa_linear_i8(const int8_t* x, int64_t x_ld, const float* x_scale, const in
  * residual, scale, gate and the norms are optional; statistics and everything between the loads and the one
  * rounding of y and of n are fp32 (n comes from the unrounded y).  With q instead of n the rows leave in 8 bits:
  *   q_scale = max |n| / 127 over the row, q = round-half-even(n / q_scale)
- * (an all-zero row: scale 0, q 0; a row holding a NaN or an infinity: scale NaN, q 0).
+ * (a row with nothing above 1.6e-36: scale 0, q 0; a row holding a NaN or an infinity: scale NaN, q 0).
  * y may be residual (same ld): in place.  No other operands may overlap.  dim <= 32768.
  */
 typedef struct sesa_norm_args {

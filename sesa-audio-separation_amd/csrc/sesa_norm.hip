@@ -156,9 +156,9 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) norm_residual_kernel(se
   }
   top = row_max<TPR>(top, red + 64);
   const float amax = __builtin_bit_cast(float, top);
-  const bool fine = top < 0x7f800000u, some = amax >= 1.6e-36f;   // (below: 127 / amax would overflow; counts as 0)
-  const float inv = fine && some ? 127.f / amax : 0.f;
-  if (t == 0) a.q_scale[row] = fine ? (some ? amax / 127.f : 0.f) : __builtin_nanf("");
+  const bool fine = top < 0x7f800000u, some = amax >= 1.6e-36f;   // (below: the scale would be subnormal; counts as 0)
+  const float scale = fine && some ? amax / 127.f : 0.f, inv = fine && some ? 1.f / scale : 0.f;
+  if (t == 0) a.q_scale[row] = fine ? scale : __builtin_nanf("");
 #pragma unroll
   for (int c = 0; c < NCH; ++c) {
     const int at = (c * TPR + t) * 8, left = dim - at;
@@ -167,8 +167,10 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) norm_residual_kernel(se
     uint32_t w[2] = {0, 0};
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      // rint of at most 127 (1 + 2^-23) in size: no clamp needed; a row without a scale stores 0
-      const int k = inv > 0.f ? (int)rintf(y[c][e] * inv) : 0;
+      // The quotient y / scale rounded to nearest, as a division gives it, from the rounded reciprocal and one correction by
+      // the exact remainder (Markstein); at most 127 (1 + 2^-23) in size: no clamp needed; a row without a scale stores 0.
+      const float g = y[c][e] * inv;
+      const int k = inv > 0.f ? (int)rintf(fmaf(fmaf(-g, scale, y[c][e]), inv, g)) : 0;
       w[e >> 2] |= (uint32_t)(k & 0xff) << (8 * (e & 3));
     }
     if (left >= 8) {

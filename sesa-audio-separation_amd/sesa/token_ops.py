@@ -472,8 +472,8 @@ def norm_residual_i8(x, residual=None, *, gate=None, gate_act="none", post="none
                      scale=None, pre="rms", pre_weight=None, pre_bias=None, eps=1e-6):
     """``norm_residual`` with n in 8 bits, one scale a row, for ``linear_i8`` -> (y, q int8, q_scale fp32 [...]).
 
-    q_scale = max |n| / 127, q = round(n / q_scale) to even.  An all-zero row has scale 0; a row that holds a NaN or an
-    infinity has scale NaN and q 0, so a product with it is NaN in every channel."""
+    q_scale = max |n| / 127, q = round(n / q_scale) to even.  A row with nothing above 1.6e-36 has scale 0; a row that holds
+    a NaN or an infinity has scale NaN and q 0, so a product with it is NaN in every channel."""
     call = _norm_residual_i8 if _eager("norm_residual_i8", x) else torch.ops.sesa.norm_residual_i8
     return call(x, residual, gate, gate_act, post, post_weight, post_bias, scale, pre, pre_weight, pre_bias, eps)
 

@@ -169,3 +169,24 @@ def test_attention_one_large_score_over_many_small_ones(d, dt, n):
     # small weights rounded to the type, exp2, n / 64 block sums and n / 16 products added in fp32, the result's rounding
     tol = m * (u + 2.0 ** -20) + (n / 64 + n / 16) * 2.0 ** -24 + u * 1.01
     assert float((got - ref).abs().max()) <= tol, (float((got - ref).abs().max()), tol, ref)
+
+
+# ---- quantize_i8 -----------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,rows,dim", [(torch.float32, 40_000, 512), (torch.float32, 3000, 1537), (torch.float16, 20_000, 1024),
+                                         (torch.bfloat16, 500, 9000)])
+@pytest.mark.parametrize("size", [1.0, 1e-30, 1e30])
+def test_quantize_i8_is_the_rounded_quotient(dt, rows, dim, size):
+    """q = round(x / q_scale) to even for every element, the quotient rounded once to fp32 (here: in 64 bits, which holds it
+    well enough that rounding it again is the same)."""
+    from sesa import ops
+    if dt == torch.float16:
+        size = min(max(size, 1e-3), 1e3)
+    x = (torch.randn(rows, dim, generator=gen(dim), device="cuda") * size).to(dt)
+    x[:, 0] = x.abs().amax(-1)                              # (a positive largest value ...)
+    step = (x[:, 0].double() / 127).float().double()         # ... and values at and beside half steps
+    for i in range(1, 100):
+        x[:, i] = ((i - 50 + 0.5) * step * (1 + (i % 3 - 1) * 2.0 ** -24)).to(dt)
+    q, s = ops.quantize_i8(x)
+    assert torch.equal(s, step.float())
+    assert torch.equal(q.double(), torch.round((x.double() / s.double()[:, None]).float().double()))
