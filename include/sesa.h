@@ -307,7 +307,8 @@ int sesa_htdemucs_destroy(sesa_htdemucs* m);
 /* Linear layer on 8-bit integers with one scale per token and one per output channel:
  *   out[m, n] = act( x_scale[m] * w_scale[n] * sum_k x[m, k] * w[n, k] + bias[n] )
  * x [m, k] and w [n, k] int8, the sum in 32-bit integers (exact for k <= 131071, the largest accepted), the scales,
- * bias (nullable) and epilogue in fp32, out rounded once to out_dtype.  A scale that is NaN makes its row / column NaN.
+ * bias (nullable) and epilogue in fp32, (sum * x_scale) first, out rounded once to out_dtype.  A scale that is NaN makes
+ * its row / column NaN; x_scale below 2^96 keeps sum * x_scale in range.
  * m < 2^31 - 256, n < 2^27.
  */
 int sesa_linear_i8(const int8_t* x, int64_t x_ld, const float* x_scale, const int8_t* w, int64_t w_ld,

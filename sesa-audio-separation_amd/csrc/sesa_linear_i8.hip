@@ -1,7 +1,8 @@
 // sesa_linear_i8: out[m, n] = act(x_scale[m] w_scale[n] sum_k x[m, k] w[n, k] + bias[n]) on 8-bit integers.
 //
 // v_mfma_i32_16x16x64_i8 with the weights as the first operand: a lane's accumulators are then consecutive output
-// channels of one token.  The sums are exact 32-bit integers; scales, bias and activation are fp32, one rounding.
+// channels of one token.  The sums are exact 32-bit integers; scales, bias and activation are fp32, one rounding.  The
+// token's scale goes to the sum first: the two scales' own product may leave the range of fp32 where the result does not.
 // Measured: one token, 4096 -> 16384 (64 MB of weights) 17.1 us, 3.9 TB/s; 8192 tokens 482 us, 2.28 POP/s.
 //
 // Two kernels:
@@ -245,7 +246,7 @@ __global__ void __launch_bounds__(WAN* WAM * 64, OCC) tile_kernel(LinArgs a) {
           const f32x4 b4 = *reinterpret_cast<const f32x4*>(b_l + c0 + 4 * j);
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            v[j >> 1][4 * (j & 1) + e] = activate<ACT>(fmaf((float)acc[u][j][i][e], xs * w4[e], b4[e]));
+            v[j >> 1][4 * (j & 1) + e] = activate<ACT>(fmaf((float)acc[u][j][i][e] * xs, w4[e], b4[e]));
         }
         if (m < a.m && left > 0) {
           TO* o = out + (int64_t)m * a.o_ld + n;
@@ -314,7 +315,7 @@ __global__ void __launch_bounds__(512) few_kernel(LinArgs a) {
       for (int e = 0; e < 4; ++e)
         if (n + e < a.n)
           out[(int64_t)m * a.o_ld + n + e] = (TO)activate<decltype(act)::value>(
-              fmaf((float)v[e], xs * a.w_scale[n + e], a.bias ? a.bias[n + e] : 0.f));
+              fmaf((float)v[e] * xs, a.w_scale[n + e], a.bias ? a.bias[n + e] : 0.f));
     }
   });
 }

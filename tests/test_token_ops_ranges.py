@@ -190,3 +190,30 @@ def test_quantize_i8_is_the_rounded_quotient(dt, rows, dim, size):
     q, s = ops.quantize_i8(x)
     assert torch.equal(s, step.float())
     assert torch.equal(q.double(), torch.round((x.double() / s.double()[:, None]).float().double()))
+
+
+# ---- linear_i8 -------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("xe,we", [(-120, -20), (-20, -120), (-100, 60), (90, -90), (95, 20), (20, 110)])
+@pytest.mark.parametrize("m", [3, 40, 300])
+def test_linear_i8_scales_at_both_ends(m, xe, we):
+    """Scales whose own product would be subnormal, or past the largest fp32 number under a sum of 0: the result is what
+    the formula gives."""
+    from sesa import ops
+    g = gen(m)
+    x, w = (torch.randint(-127, 128, (r, 200), generator=g, device="cuda", dtype=torch.int8) for r in (m, 70))
+    w[5] = 0                                                 # sums of 0
+    if xe + we > 100:                                        # ... and small ones, in range times scales as large as these
+        x[:, 1:], w[:, 1:] = 0, 0
+        x[:, 0], w[:, 0] = x[:, 0].clamp(-1, 1), w[:, 0].clamp(-1, 1)
+    xs, ws = (2.0 ** e * (1 + torch.rand(r, generator=g, device="cuda")) for r, e in ((m, xe), (70, we)))
+    for bias in (None, torch.randn(70, generator=g, device="cuda")):
+        want = (x.double() @ w.double().t()) * xs.double()[:, None] * ws.double()
+        tol = 4 * 2.0 ** -24 * want.abs()
+        if bias is not None:
+            want = want + bias.double()
+        tol = tol + 2.0 ** -24 * want.abs() + 2.0 ** -149
+        got = ops.linear_i8(x, xs, w, ws, bias, out_dtype=torch.float32)
+        big = want.abs() > 3.4e38
+        assert bool(torch.isinf(got)[big].all()) and not bool(torch.isnan(got).any())
+        assert bool(((got.double() - want).abs() <= tol)[~big].all())
