@@ -93,7 +93,9 @@ __global__ void __launch_bounds__(WAN* WAM * 64, OCC) tile_kernel(LinArgs a) {
   const int tiles_n = (a.n + BN - 1) / BN, tiles_m = (a.m + BM - 1) / BM;
   const int steps = (a.k + BK - 1) / BK;
   // within a die's range of tiles: strips of 4 token tiles, channels along the strip
-  const int t = die_tile(blockIdx.x, gridDim.x);
+  const int nb = tiles_m * tiles_n;
+  if (long_block() >= nb) return;
+  const int t = die_tile((int)long_block(), nb);
   constexpr int STRIP = 4;
   const int strip = t / (STRIP * tiles_n), in = t - strip * STRIP * tiles_n;
   const int sm = min(STRIP, tiles_m - strip * STRIP);
@@ -260,14 +262,15 @@ __global__ void __launch_bounds__(WAN* WAM * 64, OCC) tile_kernel(LinArgs a) {
 
 // ---------------------------------------------------------------------------------------------
 // Few tokens: bound by reading the weights once.  Workgroup = 16 channels x all (16 MI) tokens; NW waves take every
-// NW-th 64-byte step of K, kUnroll steps' loads in flight.
+// NW-th 64-byte step of K, U steps' loads in flight.
 template <class TO, int MI>
 __global__ void __launch_bounds__(512) few_kernel(LinArgs a) {
   constexpr int NW = 8, U = 4;   // (one token, 64 MB of weights: 17.0 us; 4 waves of 8 steps 17.9)
   __shared__ i32x4 part[NW][MI][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int l16 = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * 16;
+  if (long_block() * 16 >= a.n) return;
+  const int n0 = (int)long_block() * 16;
   const int8_t* wr = a.w + (int64_t)min(n0 + l16, a.n - 1) * a.w_ld + 16 * g;
   const int8_t* xr[MI];
 #pragma unroll
@@ -323,7 +326,7 @@ __global__ void __launch_bounds__(512) few_kernel(LinArgs a) {
 template <class TO, int WAN, int WAM, int GN, int GM, int BK, int S, int OCC>
 void launch_tile(const LinArgs& a, bool dma, hipStream_t st) {
   constexpr int BN = WAN * GN * 64, BM = WAM * GM * 16, NT = WAN * WAM * 64;
-  const dim3 grid((unsigned)((int64_t)((a.m + BM - 1) / BM) * ((a.n + BN - 1) / BN)));
+  const dim3 grid = long_grid((int64_t)((a.m + BM - 1) / BM) * ((a.n + BN - 1) / BN));
   if (dma) hipLaunchKernelGGL((tile_kernel<TO, WAN, WAM, GN, GM, BK, S, OCC, true>), grid, dim3(NT), 0, st, a);
   else hipLaunchKernelGGL((tile_kernel<TO, WAN, WAM, GN, GM, BK, S, OCC, false>), grid, dim3(NT), 0, st, a);
 }
@@ -334,7 +337,7 @@ int launch_linear(const LinArgs& a, hipStream_t st) {
   // 16 channels on the same operands are re-read so often that the 64 x 64 tile takes less (us, few | tile, k = 4096:
   // 17 x 8192 12.5 | 16.7, 17 x 16384 20.9 | 17.2, 32 x 8192 14.8 | 16.7, 64 x 4096 12.4 | 16.7, 64 x 8192 21.6 | 16.8).
   if (a.m <= 16 || (a.m <= 64 && (int64_t)((a.m + 15) / 16) * ((a.n + 15) / 16) <= 1536)) {
-    const dim3 grid((unsigned)((a.n + 15) / 16));
+    const dim3 grid = long_grid((a.n + 15) / 16);
     if (a.m <= 16) hipLaunchKernelGGL((few_kernel<TO, 1>), grid, dim3(512), 0, st, a);
     else if (a.m <= 32) hipLaunchKernelGGL((few_kernel<TO, 2>), grid, dim3(512), 0, st, a);
     else hipLaunchKernelGGL((few_kernel<TO, 4>), grid, dim3(512), 0, st, a);
@@ -378,6 +381,7 @@ extern "C" int sesa_linear_i8(const int8_t* x, int64_t x_ld, const float* x_scal
   if (m == 0) return SESA_OK;
   SESA_REQUIRE(x && x_scale && w && w_scale && out, SESA_ERR_INVALID, "linear_i8: null operand");
   SESA_REQUIRE(m == 1 || o_ld >= n, SESA_ERR_INVALID, "linear_i8: o_ld %lld is below n %d", (long long)o_ld, n);
+  // (no tile is smaller than 64 x 64 where m > 64: tile numbers fit 32 bits)
   SESA_REQUIRE((m + 63) / 64 * ((n + 63) / 64) < (1ll << 31), SESA_ERR_INVALID, "linear_i8: m x n too large");
   const LinArgs a{x, x_ld, x_scale, w, w_ld, w_scale, bias, act, (int)m, n, k, out, o_ld};
   hipStream_t st = as_stream(stream);

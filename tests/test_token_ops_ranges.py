@@ -217,3 +217,20 @@ def test_linear_i8_scales_at_both_ends(m, xe, we):
         big = want.abs() > 3.4e38
         assert bool(torch.isinf(got)[big].all()) and not bool(torch.isnan(got).any())
         assert bool(((got.double() - want).abs() <= tol)[~big].all())
+
+
+@pytest.mark.gpu
+def test_linear_i8_longest_rows_of_workgroups():
+    """As many channels, and as many tokens, as the entry takes: more threads than one grid dimension holds."""
+    from sesa import ops
+    n = 2 ** 27 - 1
+    w = torch.randint(-127, 128, (n, 1), generator=gen(1), device="cuda", dtype=torch.int8)
+    ones = torch.ones(n, device="cuda")
+    x = torch.tensor([[3], [-2]], dtype=torch.int8, device="cuda")
+    got = ops.linear_i8(x, ones[:2], w, ones)
+    assert torch.equal(got[0], (w[:, 0] * 3.0).half()) and torch.equal(got[1], (w[:, 0] * -2.0).half())
+    del got
+    m = 2 ** 27 + 1000                                       # tokens: tiles of 128 with one channel each
+    x = torch.cat([w, w[:1001]])
+    got = ops.linear_i8(x, torch.ones(m, device="cuda"), torch.full((1, 1), 5, dtype=torch.int8, device="cuda"), ones[:1])
+    assert torch.equal(got[:, 0], (x[:, 0] * 5.0).half())
