@@ -370,7 +370,8 @@ int sesa_norm_residual(const sesa_norm_args* args, void* stream);
 
 /* Rotary positions with several axes: sections[a] consecutive pairs of every head turn with axis a,
  *   (u, v) -> (u cos t - v sin t, u sin t + v cos t),  t = positions[token, a] * freqs[pair]
- * (freqs in radians per position; the angle is reduced exactly for any integer position, the rotation is fp32).
+ * (freqs in radians per position; the angle is off by at most |position| 2^-63 turns for |freq| up to 2^40, the rotation
+ * is fp32).
  * Elements from 2 P on pass through.  One or two tensors of the same tokens (q and k); out may be x with its strides.
  */
 typedef struct sesa_rope_tensor {

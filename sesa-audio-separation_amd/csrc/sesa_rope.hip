@@ -4,10 +4,10 @@
 // stores of 16-bit types), takes their sines and cosines once and applies them to its share of the heads of every tensor;
 // heads are dealt to more threads only where the tokens alone do not fill the chip.  24001 tokens, 32 + 8 heads x 128,
 // bf16: 108 us, 4.5 TB/s of the copy's 5.1; three tokens: 5.4 us on the device.
-// Angle: one turn is 2^64.  freqs / (2 pi) is reduced to a fraction of a turn in fp64 and held as a 64-bit integer,
-// so position * freq wraps modulo one turn in integer arithmetic: the phase is off by at most |position| 2^-54 turns
-// whatever the position is (an fp32 product is off by half a radian at position 10^7).  The phase's top 32 bits then go
-// to sin / cos as fp32 half-turns, off by at most 2^-25 of a half-turn.
+// Angle: one turn is 2^64.  freqs / (2 pi), with 1 / (2 pi) in two doubles, is reduced to a fraction of a turn and held as
+// a 64-bit integer, so position * freq wraps modulo one turn in integer arithmetic: the phase is off by at most |position|
+// 2^-63 turns for |freq| up to 2^40 (one double: |position| max(1, |freq| / pi) 2^-54; an fp32 product is off by half a
+// radian at position 10^7).  The phase's top 32 bits then go to sin / cos as fp32 half-turns, off by at most 2^-25 of one.
 #include "sesa_tokens.h"
 
 namespace sesa {
@@ -21,6 +21,16 @@ struct RopePlan {
   int n_all;    // ... and that copy the elements behind the pairs
   int hsplit;   // heads of each tensor are dealt round-robin to this many threads
 };
+
+// freq / (2 pi) modulo one turn in units of 2^-64 turns, rounded to an even number of them
+__device__ __forceinline__ uint64_t turn_step(float freq) {
+#pragma clang fp contract(off)   // (f as rounded: a product fused into f - rint(f) would count the remainder twice)
+  constexpr double kHi = 0x1.45f306dc9c883p-3, kLo = -0x1.6b01ec5417056p-57, kTurn = 0x1p63;   // 1 / (2 pi) = kHi + kLo
+  const double f = (double)freq * kHi, rem = fma((double)freq, kHi, -f) + (double)freq * kLo;
+  const double top = (f - rint(f)) * kTurn, whole = trunc(top);   // [-1/2, 1/2] turns: times 2^63 it fits with room
+  const double low = rint((rem - rint(rem)) * kTurn + (top - whole));
+  return ((uint64_t)(int64_t)whole + (uint64_t)(int64_t)low) << 1;
+}
 
 template <class T, bool PAIRS>
 __global__ void __launch_bounds__(256) rope_axes_kernel(sesa_rope_args a, RopePlan pl) {
@@ -59,10 +69,7 @@ __global__ void __launch_bounds__(256) rope_axes_kernel(sesa_rope_args a, RopePl
       const int64_t at = token * a.positions_ld + min(axis, a.n_axes - 1);
       const int64_t pos = a.positions_i64 ? reinterpret_cast<const int64_t*>(a.positions)[at]
                                           : reinterpret_cast<const int32_t*>(a.positions)[at];
-      const double f = (double)a.freqs[p] * 0.15915494309189533577;
-      const double frac = f - rint(f);   // [-1/2, 1/2]: times 2^63 it fits an int64 with room
-      const uint64_t step = (uint64_t)(int64_t)(frac * 9223372036854775808.0) << 1;
-      const int32_t phase = (int32_t)((step * (uint64_t)pos) >> 32);
+      const int32_t phase = (int32_t)((turn_step(a.freqs[p]) * (uint64_t)pos) >> 32);
       sincospif((float)phase * 4.656612873077392578125e-10f, &sn[i], &cs[i]);   // phase 2^-31 half-turns
     }
   }

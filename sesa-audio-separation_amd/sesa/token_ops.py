@@ -486,9 +486,9 @@ def quantize_i8(x):
 def rope_axes(q, k, positions, freqs, sections, *, layout="halves"):
     """Rotary positions with several axes on q [tokens, heads, head_dim] and k (same tokens; or None) -> (q', k') or q'.
 
-    positions int32 / int64 [tokens, axes] (any value; angles are reduced exactly), sections the number of pairs each axis
-    turns, freqs fp32 [sum(sections)] in radians per position.  layout 'halves': pair i = elements (i, i + P), P =
-    sum(sections); 'pairs': (2 i, 2 i + 1).  Elements behind the pairs pass through."""
+    positions int32 / int64 [tokens, axes] (angles are off by at most |position| 2^-63 turns), sections the number of pairs
+    each axis turns, freqs fp32 [sum(sections)] in radians per position, up to 2^40.  layout 'halves': pair i = elements
+    (i, i + P), P = sum(sections); 'pairs': (2 i, 2 i + 1).  Elements behind the pairs pass through."""
     call = _rope_axes if _eager("rope_axes", q) else torch.ops.sesa.rope_axes
     out = call([q] if k is None else [q, k], positions, freqs, sections, layout)
     return out[0] if k is None else (out[0], out[1])

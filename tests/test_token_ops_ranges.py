@@ -234,3 +234,51 @@ def test_linear_i8_longest_rows_of_workgroups():
     x = torch.cat([w, w[:1001]])
     got = ops.linear_i8(x, torch.ones(m, device="cuda"), torch.full((1, 1), 5, dtype=torch.int8, device="cuda"), ones[:1])
     assert torch.equal(got[:, 0], (x[:, 0] * 5.0).half())
+
+
+# ---- rope_axes -------------------------------------------------------------------------------------------------
+TURNS_2_200 = 255752132986241185678408580023709873616295664310550962376831   # floor(2^200 / (2 pi)), from pi to 110 digits
+
+
+def far_angles(pos, freqs):
+    """position * freq modulo one turn in whole numbers, as angles in 64 bits."""
+    rows = []
+    for p in pos:
+        row = []
+        for f in freqs:
+            num, den = float(f).as_integer_ratio()            # (an fp32 number: den a power of two)
+            row.append((p * num * TURNS_2_200 // den) % 2 ** 200 / 2 ** 200 * 2 * math.pi)
+        rows.append(row)
+    return torch.tensor(rows, dtype=torch.double)
+
+
+def test_turns_literal():
+    """pi from Machin's formula in whole numbers."""
+    one = 10 ** 110
+
+    def arctan_inverse(x):
+        t, s, k = one // x, one // x, 3
+        while t:
+            t //= -x * x
+            s += t // k
+            k += 2
+        return s
+    pi = 4 * (4 * arctan_inverse(5) - arctan_inverse(239))
+    assert abs(2 ** 200 * one // (2 * pi) - TURNS_2_200) <= 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("freq", [1e-4, 1.0, 10.0, 100.0, 1000.0, 1e6, 1e11])
+def test_rope_axes_far_positions_at_any_frequency(freq):
+    from sesa import ops
+    g = gen(5)
+    pos = [0, 1, -1, 4095, 10 ** 6, 2 ** 31 - 1, -2 ** 31, 2 ** 37 + 1, -2 ** 40, 2 ** 45 + 7]
+    freqs = freq * (1 + torch.rand(8, generator=g, device="cuda"))
+    x = torch.randn(len(pos), 2, 16, generator=g, device="cuda")
+    ang = far_angles(pos, freqs.cpu()).to("cuda")[:, None]
+    c, s, u, v = torch.cos(ang), torch.sin(ang), x[..., :8].double(), x[..., 8:].double()
+    p = torch.tensor(pos, device="cuda")[:, None]
+    ref, mag = torch.cat([u * c - v * s, u * s + v * c], -1), torch.cat([u.abs() + v.abs()] * 2, -1)
+    # angle 2^-25 half-turns off and the position's share, sine and cosine two steps, two products and a sum
+    tol = (16 * 2.0 ** -24 + 2 * math.pi * 2.0 ** -63 * p.double().abs()[:, None]) * mag + 2.0 ** -24 * ref.abs()
+    close(ops.rope_axes(x, None, p, freqs, [8]), ref, tol)
