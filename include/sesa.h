@@ -371,7 +371,7 @@ int sesa_norm_residual(const sesa_norm_args* args, void* stream);
 /* Rotary positions with several axes: sections[a] consecutive pairs of every head turn with axis a,
  *   (u, v) -> (u cos t - v sin t, u sin t + v cos t),  t = positions[token, a] * freqs[pair]
  * (freqs in radians per position; the angle is off by at most |position| 2^-63 turns for |freq| up to 2^40, the rotation
- * is fp32).
+ * is fp32; a NaN or infinite freq turns its pairs into NaN).
  * Elements from 2 P on pass through.  One or two tensors of the same tokens (q and k); out may be x with its strides.
  */
 typedef struct sesa_rope_tensor {

@@ -69,8 +69,11 @@ __global__ void __launch_bounds__(256) rope_axes_kernel(sesa_rope_args a, RopePl
       const int64_t at = token * a.positions_ld + min(axis, a.n_axes - 1);
       const int64_t pos = a.positions_i64 ? reinterpret_cast<const int64_t*>(a.positions)[at]
                                           : reinterpret_cast<const int32_t*>(a.positions)[at];
-      const int32_t phase = (int32_t)((turn_step(a.freqs[p]) * (uint64_t)pos) >> 32);
+      const float freq = a.freqs[p];
+      const bool fine = fabsf(freq) < INFINITY;   // (anything else has no integer; it turns its pair into NaN)
+      const int32_t phase = (int32_t)((turn_step(fine ? freq : 0.f) * (uint64_t)pos) >> 32);
       sincospif((float)phase * 4.656612873077392578125e-10f, &sn[i], &cs[i]);   // phase 2^-31 half-turns
+      if (!fine) cs[i] = sn[i] = __builtin_nanf("");
     }
   }
   for (int k = 0; k < a.n_tensors; ++k) {

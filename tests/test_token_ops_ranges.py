@@ -282,3 +282,21 @@ def test_rope_axes_far_positions_at_any_frequency(freq):
     # angle 2^-25 half-turns off and the position's share, sine and cosine two steps, two products and a sum
     tol = (16 * 2.0 ** -24 + 2 * math.pi * 2.0 ** -63 * p.double().abs()[:, None]) * mag + 2.0 ** -24 * ref.abs()
     close(ops.rope_axes(x, None, p, freqs, [8]), ref, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout", ["halves", "pairs"])
+def test_rope_axes_non_finite_frequencies(layout):
+    """A NaN or infinite frequency makes its own pair NaN, at every position, and nothing else."""
+    from sesa import ops
+    x = torch.randn(3, 2, 24, generator=gen(6), device="cuda")
+    pos = torch.tensor([[0], [1], [-7]], device="cuda")
+    freqs = torch.rand(10, generator=gen(7), device="cuda")
+    want = ops.rope_axes(x, None, pos, freqs, [10], layout=layout)
+    bad = [1, 4, 9]
+    freqs[bad] = torch.tensor([math.nan, math.inf, -math.inf], device="cuda")
+    at = [e for i in bad for e in ((i, 10 + i) if layout == "halves" else (2 * i, 2 * i + 1))]
+    got = ops.rope_axes(x, None, pos, freqs, [10], layout=layout)
+    assert bool(torch.isnan(got[..., at]).all())
+    rest = [e for e in range(24) if e not in at]
+    assert torch.equal(got[..., rest], want[..., rest])
