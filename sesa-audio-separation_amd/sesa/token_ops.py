@@ -14,6 +14,7 @@ share of a call is most of it.
 import ctypes
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from . import _native as N
 
@@ -83,18 +84,33 @@ def _launch(op, idx, entry, *args):
 
 
 _Tensor = torch.Tensor
+_PLAIN = {torch.Tensor, torch.nn.Parameter, type(None)}
 _compiling = torch.compiler.is_compiling
-_modes = getattr(torch._C, "_len_torch_dispatch_stack", lambda: 1)
+_tracing = torch._C._get_tracing_state
+_dispatch_modes = torch._C._len_torch_dispatch_stack
+_function_modes = torch._C._len_torch_function_stack
+_transforms = torch._C._are_functorch_transforms_active
 _current_device = torch.cuda.current_device
 _current_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _eager(op, t):
-    """Whether a call can go straight to its device kernel: a plain device tensor, nothing tracing or intercepting the
-    ops.  Saves the dispatcher's share of the host's time (3 to 4 us a call: a one-token call takes 5 to 8)."""
-    if not isinstance(t, _Tensor) or not t.is_cuda:
+def _plain(*tensors):
+    """Whether nothing but the values counts: plain tensors (or None), and no torch.compile or torch.jit trace, no torch.func
+    transform, no mode and no forward-mode level that would have to see the op."""
+    return set(map(type, tensors)) <= _PLAIN and not (_compiling() or _dispatch_modes() or _function_modes() or _transforms() or
+                                                      _tracing() is not None or _forward_ad._current_level >= 0)
+
+
+def _eager(op, t, *more):
+    """Whether a call can go straight to its device kernel: a device tensor, and ``_plain``.  Saves the dispatcher's share of
+    the host's time (3 to 4 us a call: a one-token call takes 6 to 9)."""
+    if not isinstance(t, _Tensor):
+        if hasattr(type(t), "__torch_function__"):   # a stand-in (torch.fx): the op itself goes into its graph
+            return False
         _device(op, t)
-    return type(t) is _Tensor and not _compiling() and not _modes()
+    elif not t.is_cuda:
+        _device(op, t)
+    return _plain(t, *more)
 
 
 def _param(op, name, t, n):
@@ -451,7 +467,7 @@ def linear_i8(x, x_scale, weight, w_scale, bias=None, *, act="none", out_dtype=t
     x int8 [..., k] with x_scale fp32 [...] (one scale a token), weight int8 [n, k] with w_scale fp32 [n] (one a channel;
     ``quantize_i8`` makes both pairs), bias fp32 [n] or None; act 'none', 'gelu' (erf), 'tanh' or 'relu'.  The sum is an
     exact 32-bit integer (k <= 131071), everything after it fp32, rounded once."""
-    call = _linear_i8 if _eager("linear_i8", x) else torch.ops.sesa.linear_i8
+    call = _linear_i8 if _eager("linear_i8", x, x_scale, weight, w_scale, bias) else torch.ops.sesa.linear_i8
     return call(x, x_scale, weight, w_scale, bias, act, out_dtype)
 
 
@@ -464,7 +480,8 @@ def norm_residual(x, residual=None, *, gate=None, gate_act="none", post="none", 
     gate that many rows share ([groups, dim] for x [rows, dim]); gate_act 'none', 'sigmoid', 'silu' or 'tanh'.
     post / pre: 'none', 'rms' or 'layer' with fp32 [dim] weights (None: 1) and biases (None: 0); scale fp32 [dim].
     Statistics are fp32; y and n are rounded once, n from the unrounded y."""
-    call = _norm_residual if _eager("norm_residual", x) else torch.ops.sesa.norm_residual
+    eager = _eager("norm_residual", x, residual, gate, post_weight, post_bias, scale, pre_weight, pre_bias)
+    call = _norm_residual if eager else torch.ops.sesa.norm_residual
     return call(x, residual, gate, gate_act, post, post_weight, post_bias, scale, pre, pre_weight, pre_bias, eps)
 
 
@@ -474,7 +491,8 @@ def norm_residual_i8(x, residual=None, *, gate=None, gate_act="none", post="none
 
     q_scale = max |n| / 127, q = round(n / q_scale) to even.  A row with nothing above 1.6e-36 has scale 0; a row that holds
     a NaN or an infinity has scale NaN and q 0, so a product with it is NaN in every channel."""
-    call = _norm_residual_i8 if _eager("norm_residual_i8", x) else torch.ops.sesa.norm_residual_i8
+    eager = _eager("norm_residual_i8", x, residual, gate, post_weight, post_bias, scale, pre_weight, pre_bias)
+    call = _norm_residual_i8 if eager else torch.ops.sesa.norm_residual_i8
     return call(x, residual, gate, gate_act, post, post_weight, post_bias, scale, pre, pre_weight, pre_bias, eps)
 
 
@@ -489,14 +507,14 @@ def rope_axes(q, k, positions, freqs, sections, *, layout="halves"):
     positions int32 / int64 [tokens, axes] (angles are off by at most |position| 2^-63 turns), sections the number of pairs
     each axis turns, freqs fp32 [sum(sections)] in radians per position, up to 2^40.  layout 'halves': pair i = elements
     (i, i + P), P = sum(sections); 'pairs': (2 i, 2 i + 1).  Elements behind the pairs pass through."""
-    call = _rope_axes if _eager("rope_axes", q) else torch.ops.sesa.rope_axes
+    call = _rope_axes if _eager("rope_axes", q, k, positions, freqs) else torch.ops.sesa.rope_axes
     out = call([q] if k is None else [q, k], positions, freqs, sections, layout)
     return out[0] if k is None else (out[0], out[1])
 
 
 def rope_axes_(q, k, positions, freqs, sections, *, layout="halves"):
     """``rope_axes`` in place on q and k (k may be None)."""
-    _device("rope_axes_", q)
+    _eager("rope_axes_", q)
     torch.ops.sesa.rope_axes_([q] if k is None else [q, k], positions, freqs, sections, layout)
 
 
@@ -511,7 +529,7 @@ def attention_packed(q, k, v, cu_seqlens=None, *, causal=True, scale=None, gate=
     is taken as the run's end, and boundaries out of order give unspecified rows, never an access outside.  gate: logits [tokens, (lanes,) heads], a sigmoid on each head's output.  scale: head_dim ** -0.5.
     Rows of no sequence (behind the last) come back 0; with ``out`` they are left as they were.  Infinite or NaN values
     and scores beyond 2.9e6 give what the formula says, but such rows go key by key (``include/sesa.h``), slowly."""
-    eager = _eager("attention_packed", q)
+    eager = _eager("attention_packed", q, k, v, cu_seqlens, gate)
     if out is None:
         call = _attention_packed if eager else torch.ops.sesa.attention_packed
         return call(q, k, v, cu_seqlens, causal, scale, gate)

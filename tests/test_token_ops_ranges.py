@@ -300,3 +300,111 @@ def test_rope_axes_non_finite_frequencies(layout):
     assert bool(torch.isnan(got[..., at]).all())
     rest = [e for e in range(24) if e not in at]
     assert torch.equal(got[..., rest], want[..., rest])
+
+
+# ---- traced, transformed and intercepted calls ----------------------------------------------------------------
+def test_the_direct_path_is_for_plain_calls_only():
+    """What sends a call through the registered op instead of straight to its kernel."""
+    from torch.autograd import forward_ad
+    from torch.overrides import TorchFunctionMode
+    from torch.utils._python_dispatch import TorchDispatchMode
+    from sesa.token_ops import _plain
+    x = torch.zeros(2, 4)
+    assert _plain(x, None, torch.nn.Parameter(x))
+    assert not _plain(x, x.as_subclass(type("Mine", (torch.Tensor,), {})))
+
+    class Dispatch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    class Function(TorchFunctionMode):
+        def __torch_function__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+    for mode in (Dispatch(), Function(), forward_ad.dual_level()):
+        with mode:
+            assert not _plain(x)
+    seen = []
+
+    def look(t):
+        seen.append(_plain(t))
+        return t * 2
+    torch.jit.trace(look, (x,), check_trace=False)   # (the check is a plain call)
+    torch.func.vmap(look)(x)
+    torch.func.grad(lambda t: look(t).sum())(x)
+    torch.func.jvp(look, (x,), (x,))
+    assert len(seen) >= 4 and not any(seen)
+    assert _plain(x)
+
+
+def test_fx_records_the_ops():
+    from sesa import ops
+
+    def f(x, xs, w, ws, q, k, pos, freqs, cu):
+        a, b = ops.rope_axes(q, k, pos, freqs, [8])
+        ops.rope_axes_(a, b, pos, freqs, [8])
+        y, n = ops.norm_residual(x)
+        y, q8, s = ops.norm_residual_i8(n, y)
+        return ops.linear_i8(x, xs, w, ws), ops.attention_packed(a, b, b, cu), ops.quantize_i8(y)
+    graph = torch.fx.symbolic_trace(f).graph
+    names = [str(n.target) for n in graph.nodes if n.op == "call_function"]
+    for op in ("linear_i8", "norm_residual", "norm_residual_i8", "quantize_i8", "rope_axes", "rope_axes_", "attention_packed"):
+        assert any(n.split(".")[-1] == op or n.endswith(f"sesa.{op}") for n in names), (op, names)
+
+
+@pytest.fixture
+def some():
+    """Small inputs of every operator, by seed."""
+    def make(seed):
+        g = gen(seed)
+        r = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+        return dict(x=r(6, 32).half(), res=r(6, 32), w=r(24, 32), qkv=r(6, 4, 16).half(),
+                    pos=torch.randint(0, 99, (6, 1), generator=g, device="cuda"), freqs=r(8))
+    return make
+
+
+def all_ops(x, res, w, qkv, pos, freqs):
+    from sesa import ops
+    y, n = ops.norm_residual(x, res)
+    y8, q8, s = ops.norm_residual_i8(x, res, pre="layer")
+    out = ops.linear_i8(q8, s, *ops.quantize_i8(w), act="gelu")
+    a, b = ops.rope_axes(qkv[:, :2], qkv[:, 2:3], pos, freqs, [8])
+    return y, n, y8, q8, s, out, a, b, ops.attention_packed(a, b, qkv[:, 3:])
+
+
+@pytest.mark.gpu
+def test_jit_trace(some):
+    """A traced function computes: new inputs give what the eager call gives."""
+    names = list(some(0))
+    traced = torch.jit.trace(lambda *a: all_ops(*a), tuple(some(1)[n] for n in names), check_trace=False)
+    assert "sesa::linear_i8" in str(traced.graph) and "sesa::attention_packed" in str(traced.graph)
+    for seed in (2, 3):
+        args = [some(seed)[n] for n in names]
+        junk = [torch.full((1 << 18,), math.nan, device="cuda") for _ in range(8)]   # (what an unwritten result would hold)
+        del junk
+        for a, b in zip(traced(*args), all_ops(*args)):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_vmap_and_function_modes(some):
+    from torch.overrides import TorchFunctionMode
+    from sesa import ops
+    sets = [some(s) for s in (4, 5, 6)]
+    x, res, w = (torch.stack([s[n] for s in sets]) for n in ("x", "res", "w"))
+    want = [ops.norm_residual_i8(s["x"], s["res"]) for s in sets]
+    for a, b in zip(torch.func.vmap(lambda x, r: ops.norm_residual_i8(x, r))(x, res), zip(*want)):
+        assert torch.equal(a, torch.stack(b))
+    w8, ws = ops.quantize_i8(w)
+    y = torch.func.vmap(lambda x, w, ws: ops.linear_i8(*ops.quantize_i8(x), w, ws))(x, w8, ws)
+    assert all(torch.equal(y[i], ops.linear_i8(*ops.quantize_i8(x[i]), w8[i], ws[i])) for i in range(3))
+    seen = []
+
+    class Watch(TorchFunctionMode):
+        def __torch_function__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+    with Watch():
+        got = all_ops(**sets[0])
+    assert all(torch.equal(a, b) for a, b in zip(got, all_ops(**sets[0])))
+    for op in ("linear_i8", "norm_residual", "norm_residual_i8", "quantize_i8", "rope_axes", "attention_packed"):
+        assert any(s.endswith(f"sesa.{op}") for s in seen), (op, seen)
