@@ -7,9 +7,9 @@ and residual between two blocks; rows in 8 bits), ``rope_axes`` / ``rope_axes_``
 
 Device tensors only, on the current stream of the tensors' device; every result is a new tensor unless the name says
 otherwise; nothing waits for the device, so the calls can be captured into a graph.  Inference only: a call whose
-inputs would need a gradient raises.  The ops are plain ``torch.library`` definitions (schema, device kernel, fake
-kernel), and an eager call of the functions below goes straight to the device kernel: for a single token the host's
-share of a call is most of it.
+inputs would need a gradient, backward or forward mode, raises, also while it is compiled.  The ops are plain
+``torch.library`` definitions (schema, device kernel, fake kernel, an autograd kernel that refuses), and a plain eager call
+of the functions below goes straight to the device kernel: for a single token the host's share of a call is most of it.
 """
 import ctypes
 
@@ -29,18 +29,39 @@ _LIB = torch.library.Library("sesa", "FRAGMENT")
 
 
 def _define(schema):
-    """Registers ``schema`` with the decorated function as its device kernel."""
+    """Registers ``schema`` with the decorated function as its device kernel, and the refusal of gradients above it."""
     name = schema.split("(", 1)[0]
 
     def wrap(fn):
         _LIB.define(schema)
         _LIB.impl(name, fn, "CUDA")
+        op = getattr(torch.ops.sesa, name).default
+        args = [a.name for a in op._schema.arguments]
+
+        def forward_only(*values):
+            _refuse_gradients(name, args, values)
+            with torch._C._AutoDispatchBelowAutograd():
+                return op(*values)
+        _LIB.impl(name, forward_only, "Autograd")
         return fn
     return wrap
 
 
 def _fail(op, msg):
     raise N.SesaError(f"sesa::{op}: {msg}")
+
+
+def _refuse_gradients(op, names, values):
+    """No argument waits for a gradient or carries a forward-mode tangent.  The dispatcher asks this where autograd would
+    record the op, so a compiled graph is refused while it is traced (its own run has gradients off)."""
+    grad, forward = torch.is_grad_enabled(), _forward_ad._current_level >= 0
+    if not grad and not forward:
+        return
+    for name, value in zip(names, values):
+        for t in value if isinstance(value, (list, tuple)) else (value,):
+            if isinstance(t, torch.Tensor) and (grad and t.requires_grad or
+                                                forward and _forward_ad.unpack_dual(t).tangent is not None):
+                _fail(op, f"{name} requires a gradient and this operator has none (use torch.no_grad())")
 
 
 def _check(op, idx, names, *tensors):

@@ -408,3 +408,80 @@ def test_vmap_and_function_modes(some):
     assert all(torch.equal(a, b) for a, b in zip(got, all_ops(**sets[0])))
     for op in ("linear_i8", "norm_residual", "norm_residual_i8", "quantize_i8", "rope_axes", "attention_packed"):
         assert any(s.endswith(f"sesa.{op}") for s in seen), (op, seen)
+
+
+# ---- gradients: refused, however the call is made --------------------------------------------------------------
+def op_calls(dev):
+    """(name, call of the op with one of its tensors in place of x) for every operator; the rest on ``dev``."""
+    z = lambda *s, dt=torch.float16: torch.zeros(*s, dtype=dt, device=dev)  # noqa: E731
+    i8 = torch.int8
+    O = torch.ops.sesa  # noqa: N806
+    rest = (None, "none", "none", None, None, None, "rms", None, None, 1e-6)
+    pos = z(2, 1, dt=torch.int32)
+    return [
+        ("linear_i8", z(2, dt=torch.float32), lambda x: O.linear_i8(z(2, 16, dt=i8), x, z(4, 16, dt=i8), z(4, dt=torch.float32), None,
+                                                                   "none", torch.float32)),
+        ("norm_residual", z(2, 8), lambda x: O.norm_residual(x, None, *rest)[0]),
+        ("norm_residual", z(2, 8), lambda x: O.norm_residual(z(2, 8), x, *rest)[0]),
+        ("norm_residual_i8", z(2, 8), lambda x: O.norm_residual_i8(x, None, *rest)[0]),
+        ("quantize_i8", z(2, 8), lambda x: O.quantize_i8(x)[1]),
+        ("rope_axes", z(2, 1, 8), lambda x: O.rope_axes([z(2, 1, 8), x], pos, z(4, dt=torch.float32), [4], "halves")[0]),
+        ("rope_axes", z(4, dt=torch.float32), lambda x: O.rope_axes([z(2, 1, 8)], pos, x, [4], "halves")[0]),
+        ("rope_axes_", z(4, dt=torch.float32), lambda x: O.rope_axes_([z(2, 1, 8)], pos, x, [4], "halves")),
+        ("attention_packed", z(2, 1, 8), lambda x: O.attention_packed(x, x, x, None, True, None, None)),
+        ("attention_packed", z(2, 1), lambda x: O.attention_packed(z(2, 1, 8), z(2, 1, 8), z(2, 1, 8), None, True, None, x)),
+        ("attention_packed_into", z(2, 1, 8), lambda x: O.attention_packed_into(x, x, x, None, True, None, None, z(2, 1, 8))),
+    ]
+
+
+def refuse_gradients(dev):
+    from torch.autograd import forward_ad
+    from sesa import ops  # noqa: F401
+    from sesa._native import SesaError
+    for name, t, call in op_calls(dev):
+        with pytest.raises(SesaError, match=f"{name}: .* requires a gradient"):
+            call(t.clone().requires_grad_())
+        for grad_of in (lambda x: torch.func.grad(lambda y: call(y).float().sum())(x), lambda x: torch.func.jvp(call, (x,), (x,))):
+            with pytest.raises(SesaError, match=f"{name}: .* requires a gradient"):
+                grad_of(t)
+        with forward_ad.dual_level(), pytest.raises(SesaError, match=f"{name}: .* requires a gradient"):
+            call(forward_ad.make_dual(t, torch.ones_like(t)))
+
+
+def test_gradients_are_refused_by_every_op():
+    refuse_gradients("cpu")
+
+
+def test_gradients_are_refused_while_compiling():
+    from sesa import ops  # noqa: F401
+    for backend in ("eager", "aot_eager"):
+        for name, t, call in op_calls("cpu"):
+            torch._dynamo.reset()
+            out = []
+
+            def f(x):
+                y = call(x * 2)
+                return x if y is None else y * 1.0
+            with pytest.raises(Exception, match=f"{name}: .* requires a gradient"):
+                out.append(torch.compile(f, backend=backend, fullgraph=True)(t.clone().requires_grad_()))
+            assert not out
+
+
+@pytest.mark.gpu
+def test_gradients_are_refused_on_the_device(some):
+    from torch.autograd import forward_ad
+    from sesa import ops
+    from sesa._native import SesaError
+    refuse_gradients("cuda")
+    x = torch.randn(4, 32, device="cuda")
+    with forward_ad.dual_level(), pytest.raises(SesaError, match="requires a gradient"):
+        ops.norm_residual(forward_ad.make_dual(x, x))
+    w = torch.nn.Parameter(torch.ones(32, device="cuda"))
+    f = torch.compile(lambda x: ops.norm_residual(x, pre_weight=w)[1] * 2, backend="aot_eager", fullgraph=True)
+    with pytest.raises(Exception, match="requires a gradient"):
+        f(x)
+    with torch.no_grad():                       # ... and with gradients off the same call runs
+        torch._dynamo.reset()
+        assert torch.equal(f(x), ops.norm_residual(x, pre_weight=w)[1] * 2)
+    with torch.inference_mode():
+        assert torch.equal(ops.norm_residual(x.clone(), pre_weight=w)[1], f(x) / 2)
