@@ -111,6 +111,7 @@ _tracing = torch._C._get_tracing_state
 _dispatch_modes = torch._C._len_torch_dispatch_stack
 _function_modes = torch._C._len_torch_function_stack
 _transforms = torch._C._are_functorch_transforms_active
+_written = torch.autograd.graph.increment_version   # (an op saved such a tensor for its backward: that has to notice)
 _current_device = torch.cuda.current_device
 _current_stream = torch._C._cuda_getCurrentRawStream
 
@@ -406,6 +407,7 @@ def _rope_axes_(xs, positions, freqs, sections, layout):
     if len(xs) == 2 and not _apart(*xs):
         _fail("rope_axes_", "the two tensors overlap")
     _rope_call("rope_axes_", xs, xs, positions, freqs, sections, layout)
+    _written(xs)
 
 
 @torch.library.register_fake("sesa::rope_axes_", lib=_LIB)
@@ -474,6 +476,7 @@ def _attention_packed_into(q, k, v, cu_seqlens, causal, scale, gate, out):
         _fail(op, f"out: rows have to lie apart, contiguous in the last dimension; got {list(out.shape)} with strides "
                   f"{list(out.stride())}")
     _attn_call(op, q, k, v, cu_seqlens, causal, scale, gate, out, False)
+    _written(out)
 
 
 @torch.library.register_fake("sesa::attention_packed_into", lib=_LIB)
@@ -535,8 +538,8 @@ def rope_axes(q, k, positions, freqs, sections, *, layout="halves"):
 
 def rope_axes_(q, k, positions, freqs, sections, *, layout="halves"):
     """``rope_axes`` in place on q and k (k may be None)."""
-    _eager("rope_axes_", q)
-    torch.ops.sesa.rope_axes_([q] if k is None else [q, k], positions, freqs, sections, layout)
+    call = _rope_axes_ if _eager("rope_axes_", q, k, positions, freqs) else torch.ops.sesa.rope_axes_
+    call([q] if k is None else [q, k], positions, freqs, sections, layout)
 
 
 def attention_packed(q, k, v, cu_seqlens=None, *, causal=True, scale=None, gate=None, out=None):
@@ -550,9 +553,9 @@ def attention_packed(q, k, v, cu_seqlens=None, *, causal=True, scale=None, gate=
     is taken as the run's end, and boundaries out of order give unspecified rows, never an access outside.  gate: logits [tokens, (lanes,) heads], a sigmoid on each head's output.  scale: head_dim ** -0.5.
     Rows of no sequence (behind the last) come back 0; with ``out`` they are left as they were.  Infinite or NaN values
     and scores beyond 2.9e6 give what the formula says, but such rows go key by key (``include/sesa.h``), slowly."""
-    eager = _eager("attention_packed", q, k, v, cu_seqlens, gate)
+    eager = _eager("attention_packed", q, k, v, cu_seqlens, gate, out)
     if out is None:
         call = _attention_packed if eager else torch.ops.sesa.attention_packed
         return call(q, k, v, cu_seqlens, causal, scale, gate)
-    torch.ops.sesa.attention_packed_into(q, k, v, cu_seqlens, causal, scale, gate, out)
+    (_attention_packed_into if eager else torch.ops.sesa.attention_packed_into)(q, k, v, cu_seqlens, causal, scale, gate, out)
     return out

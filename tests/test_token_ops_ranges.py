@@ -485,3 +485,25 @@ def test_gradients_are_refused_on_the_device(some):
         assert torch.equal(f(x), ops.norm_residual(x, pre_weight=w)[1] * 2)
     with torch.inference_mode():
         assert torch.equal(ops.norm_residual(x.clone(), pre_weight=w)[1], f(x) / 2)
+
+
+@pytest.mark.gpu
+def test_tensors_written_in_place_count_a_version(some):
+    """An op that saved the tensor for its backward notices that it changed, also under no_grad and through the op."""
+    from sesa import ops
+    s = some(8)
+    for call in (ops.rope_axes_, lambda q, k, *a: torch.ops.sesa.rope_axes_([q, k], *a, "halves")):
+        leaf = torch.ones(6, 2, 16, device="cuda", requires_grad=True)
+        q, k = torch.randn(6, 2, 16, device="cuda"), torch.randn(6, 1, 16, device="cuda")
+        y = (leaf * q).sum()
+        with torch.no_grad():
+            call(q, k, s["pos"], s["freqs"], [8])
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+        assert k._version == 1
+    q, k, v = s["qkv"].split([2, 1, 1], 1)
+    for call in (lambda o: ops.attention_packed(q, k, v, out=o),
+                 lambda o: torch.ops.sesa.attention_packed_into(q, k, v, None, True, None, None, o)):
+        out = torch.zeros(6, 2, 16, device="cuda", dtype=torch.float16)
+        call(out)
+        assert out._version == 1 and torch.equal(out, ops.attention_packed(q, k, v))
