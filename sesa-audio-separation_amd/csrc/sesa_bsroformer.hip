@@ -317,7 +317,8 @@ int add_param(sesa_bsr* m, const std::string& name, std::vector<int64_t> shape) 
 
 const std::vector<float>& P(sesa_bsr* m, const std::string& name) { return m->params[m->by_name.at(name)].host; }
 
-// One 8-bit Linear: every row (output channel) on its own scale max |w| / 127, rounded half to even.
+// One 8-bit Linear: every row (output channel) on its own scale max |w| / 127, the quotient rounded half to even -- the rule
+// of sesa_norm_residual's 8-bit rows: nothing above 1.6e-36 is a row of zeros, a NaN or an infinity makes the scale NaN.
 template <class RowFn>
 LinI8 pack_i8(int n, int k, RowFn row_val, std::vector<int8_t>& w8, std::vector<float>& f8) {
   LinI8 l;
@@ -330,13 +331,16 @@ LinI8 pack_i8(int n, int k, RowFn row_val, std::vector<int8_t>& w8, std::vector<
   std::vector<float> row(k);
   for (int r = 0; r < n; ++r) {
     float top = 0.f;
+    bool fine = true;
     for (int i = 0; i < k; ++i) {
       row[i] = row_val(r, i);
+      fine = fine && std::isfinite(row[i]);
       top = std::max(top, std::fabs(row[i]));
     }
-    const float inv = top > 0.f ? 127.f / top : 0.f;
-    for (int i = 0; i < k; ++i) w8[l.w_off + (int64_t)r * k + i] = (int8_t)std::nearbyint(row[i] * inv);
-    f8.push_back(top / 127.f);
+    const float scale = fine && top >= 1.6e-36f ? top / 127.f : 0.f;
+    for (int i = 0; i < k; ++i)
+      w8[l.w_off + (int64_t)r * k + i] = scale > 0.f ? (int8_t)std::nearbyint(row[i] / scale) : (int8_t)0;
+    f8.push_back(fine ? scale : NAN);
   }
   return l;
 }
