@@ -69,8 +69,8 @@ def build_parser():
     p.add_argument("--exec_batch", type=int, default=0,
                    help="chunks per native forward (MI355X only; 0 = planned from the model and free HBM)")
     p.add_argument("--precision", type=str, default=None,
-                   help="the model's precision by name (MI355X only; e.g. int8 for the Roformers: 8-bit Linears, about "
-                        "1 %% error a layer); default: --enable_amp's choice")
+                   help="the model's precision by name (MI355X only; e.g. int8 for the Roformers: 8-bit Linears, 1.4 to "
+                        "1.8 %% off in all); default: --enable_amp's choice")
     return p
 
 
