@@ -348,15 +348,19 @@ int launch_linear(const LinArgs& a, hipStream_t st) {
                    (uintptr_t)a.w % 16 == 0;
   auto tiles = [&](int bm, int bn) { return (int64_t)((a.m + bm - 1) / bm) * ((a.n + bn - 1) / bn); };
   // The largest tile that still gives every compute unit a workgroup: operands are read from LDS 0.75 (256 x 256), 1
-  // (128 x 128) and 2.5 (64 x 64) times per 16-deep product.  Up to K = 512 a tile has so few steps that its
+  // (128 x 128) and 2.5 (64 x 64) times per 16-deep product.  Up to K = 640 a tile has so few steps that its
   // epilogue and first loads take longer than its products: 128 x 128 in 64-byte steps leaves room for more workgroups
-  // a CU, which hide each other's.  Measured (us, fp16 out; 256 | 128 | 128 at 64 bytes | 64):
-  //   49662 x 512 x 2048 GELU 154 | 143 | 119 | 172    8192 x 4096 x 16384  495 | 575 | 675 | 878
-  //   4096 x 1024 x 4096       22 |  28 |  29 |  36    2048 x 2048 x 2048    30 |  15 |  20 |  18
-  //   777 x 1008 x 1537 GELU   25 |  12 |  14 | 9.4    256 x 4096 x 4096     51 |  24 |  33 |  17
+  // a CU, which hide each other's.  That border, many tokens (us, fp16 out; 256 | 128 | 128 at 64 bytes):
+  //   49662 x K x 2048 GELU   K 512  130 | 112 | 102   576  142 | 130 | 112   640  138 | 125 | 119   1024  169 | 168 | 161
+  //   49662 x K x 2048        K 512   96 |  91 |  87   576  111 | 104 |  96   640  108 | 103 | 103    768  118 | 116 | 122
+  //   20000 x K x 1024 GELU   K 512   36 |  27 |  26   576   40 |  31 |  28   640   39 |  31 |  29   1024   47 |  38 |  38
+  // Sizes apart (256 | 128 | 128 at 64 bytes | 64):
+  //   8192 x 4096 x 16384     495 | 575 | 675 | 878    4096 x 1024 x 4096    22 |  28 |  29 |  36
+  //   2048 x 2048 x 2048       30 |  15 |  20 |  18    256 x 4096 x 4096     51 |  24 |  33 |  17
+  //   777 x 1008 x 1537 GELU   25 |  12 |  14 | 9.4
   // The large ones run at the rate the chip sustains on int8 products (8192^3: 2.38 PFLOP/s; MFMA busy 49 % of the
   // cycles at about 2.06 GHz); a ring deeper than two stages helps only the 64 x 64 tile (19 -> 17 us at 256 x 4096^2).
-  if (a.k <= 512 && tiles(128, 128) >= 1024) launch_tile<TO, 2, 2, 1, 4, 64, 2, 3>(a, dma, st);
+  if (a.k <= 640 && tiles(128, 128) >= 1024) launch_tile<TO, 2, 2, 1, 4, 64, 2, 3>(a, dma, st);
   else if (tiles(256, 256) >= 256) launch_tile<TO, 2, 4, 2, 4, 128, 2, 2>(a, dma, st);
   else if (tiles(128, 128) >= 256) launch_tile<TO, 2, 2, 1, 4, 128, 2, 2>(a, dma, st);
   else launch_tile<TO, 1, 4, 1, 1, 128, 4, 2>(a, dma, st);

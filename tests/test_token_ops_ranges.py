@@ -507,3 +507,13 @@ def test_tensors_written_in_place_count_a_version(some):
         out = torch.zeros(6, 2, 16, device="cuda", dtype=torch.float16)
         call(out)
         assert out._version == 1 and torch.equal(out, ops.attention_packed(q, k, v))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("k", [512, 520, 640, 648, 656, 1000])
+@pytest.mark.parametrize("m,n", [(8200, 2064), (40_000, 520)])
+def test_linear_i8_either_side_of_the_short_k_rule(m, n, k):
+    from sesa import ops
+    from test_token_ops import linear_case, linear_check
+    x, xs, w, ws, b = linear_case(m + k, m, k, n)
+    linear_check(ops.linear_i8(x, xs, w, ws, b, act="gelu", out_dtype=torch.float32), x, xs, w, ws, b, "gelu")
