@@ -11,7 +11,7 @@
 // a lane (~1000 cycles) against 512 (head 64) or 1024 (head 128) cycles of products.  Measured: 12289 causal tokens,
 // 32 / 8 heads x 128, bf16 357-417 us by the sequences' lengths (0.93-1.05 PFLOP/s of its pairs); 2 x 801 tokens x 62
 // lanes, 8 heads x 64, fp16 259-268 us (0.63 PFLOP/s: 13 blocks a tile, one of them masked, 89 % of the query rows used).
-#include "sesa_tokens.h"
+#include "sesa_tokens.hpp"
 
 namespace sesa {
 namespace {

@@ -9,7 +9,7 @@
 //  * tile_kernel: BM tokens x BN channels per workgroup, K in 128-byte steps through a ring of LDS stages.
 //  * few_kernel (m <= 16, and to 64 with few channels): 16 channels per workgroup, the waves split K and read both operands straight into the
 //    matrix instruction's registers; joined in LDS.
-#include "sesa_tokens.h"
+#include "sesa_tokens.hpp"
 
 namespace sesa {
 namespace {

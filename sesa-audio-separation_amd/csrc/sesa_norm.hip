@@ -5,7 +5,7 @@
 // 1024 above: a thread keeps at most 32 values and enough rows are in flight to cover the loads (16384 x 8192 bf16,
 // sandwich norms and gate: 334 us at 256 threads, 278 at 512, 275 at 1024; 16384 x 4096: 134, 139, -).  Statistics are two-pass over the registers (mean, then squared deviations), so LayerNorm does not
 // cancel.
-#include "sesa_tokens.h"
+#include "sesa_tokens.hpp"
 
 namespace sesa {
 namespace {

@@ -8,7 +8,7 @@
 // a 64-bit integer, so position * freq wraps modulo one turn in integer arithmetic: the phase is off by at most |position|
 // 2^-63 turns for |freq| up to 2^40 (one double: |position| max(1, |freq| / pi) 2^-54; an fp32 product is off by half a
 // radian at position 10^7).  The phase's top 32 bits then go to sin / cos as fp32 half-turns, off by at most 2^-25 of one.
-#include "sesa_tokens.h"
+#include "sesa_tokens.hpp"
 
 namespace sesa {
 namespace {

@@ -517,3 +517,22 @@ def test_linear_i8_either_side_of_the_short_k_rule(m, n, k):
     from test_token_ops import linear_case, linear_check
     x, xs, w, ws, b = linear_case(m + k, m, k, n)
     linear_check(ops.linear_i8(x, xs, w, ws, b, act="gelu", out_dtype=torch.float32), x, xs, w, ws, b, "gelu")
+
+
+# ---- the build -----------------------------------------------------------------------------------------------------
+def test_makefile_builds_every_declared_symbol():
+    """The one Makefile names every source, and the library it links has every entry that the bindings declare."""
+    import glob
+    import os
+    import subprocess
+    import sesa
+    from sesa import _native
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(sesa.__file__))), "csrc")
+    dry = subprocess.run(["make", "-f", "Makefile", "-n", "-B"], cwd=csrc, capture_output=True, text=True, check=True).stdout
+    sources = [os.path.basename(f) for f in glob.glob(os.path.join(csrc, "*.hip")) + glob.glob(os.path.join(csrc, "*.cpp"))]
+    assert len(sources) >= 16
+    for src in sources:
+        assert f"-c {src} " in dry, src
+        assert f"build/{src}.o" in dry.split("-shared")[1], src
+    lib = _native.lib()
+    assert all(hasattr(lib, name) for name in _native.SIGNATURES)
