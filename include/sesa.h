@@ -347,7 +347,8 @@ typedef struct sesa_norm_args {
   int64_t rows_per_gate;
   int gate_act;               /* SESA_GATE_*                                                             */
   int post;                   /* SESA_NORM_* of x                                                        */
-  const float* post_weight;   /* [dim] fp32, nullable: 1 (also the other parameter vectors)              */
+  const float* post_weight;   /* [dim] fp32, nullable: 1 (also the other parameter vectors); a norm that is
+                                 SESA_NORM_NONE does not read its own                                    */
   const float* post_bias;     /* nullable: 0                                                             */
   const float* scale;         /* nullable: 1                                                             */
   int pre;                    /* SESA_NORM_* of y                                                        */

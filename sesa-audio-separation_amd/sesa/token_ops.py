@@ -12,6 +12,7 @@ inputs would need a gradient, backward or forward mode, raises, also while it is
 of the functions below goes straight to the device kernel: for a single token the host's share of a call is most of it.
 """
 import ctypes
+import math
 
 import torch
 from torch.autograd import forward_ad as _forward_ad
@@ -147,7 +148,7 @@ def _param(op, name, t, n):
 def _rows(t):
     """[..., n] as [rows, n] with the last dimension contiguous (a copy only where the strides need one)."""
     if t.dim() != 2:
-        t = t.reshape(-1, t.shape[-1])
+        t = t.reshape(math.prod(t.shape[:-1]), t.shape[-1])   # (-1 has no answer where n is 0)
     return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
 
 
@@ -502,7 +503,8 @@ def norm_residual(x, residual=None, *, gate=None, gate_act="none", post="none", 
     x [..., dim] fp32 / fp16 / bf16 is a block's output, residual (same shape; x's type or fp32) the stream it joins: y
     comes in residual's type, n in x's.  gate: x's type and shape, with 1 in trailing dimensions before the last for a
     gate that many rows share ([groups, dim] for x [rows, dim]); gate_act 'none', 'sigmoid', 'silu' or 'tanh'.
-    post / pre: 'none', 'rms' or 'layer' with fp32 [dim] weights (None: 1) and biases (None: 0); scale fp32 [dim].
+    post / pre: 'none', 'rms' or 'layer' with fp32 [dim] weights (None: 1) and biases (None: 0), which 'none' does not use;
+    scale fp32 [dim].
     Statistics are fp32; y and n are rounded once, n from the unrounded y."""
     eager = _eager("norm_residual", x, residual, gate, post_weight, post_bias, scale, pre_weight, pre_bias)
     call = _norm_residual if eager else torch.ops.sesa.norm_residual

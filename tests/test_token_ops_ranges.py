@@ -536,3 +536,21 @@ def test_makefile_builds_every_declared_symbol():
         assert f"build/{src}.o" in dry.split("-shared")[1], src
     lib = _native.lib()
     assert all(hasattr(lib, name) for name in _native.SIGNATURES)
+
+
+# ---- rows without elements ---------------------------------------------------------------------------------------
+def test_rows_without_elements():
+    from sesa.token_ops import _rows
+    for shape, rows in (((2, 3, 0), 6), ((0, 5, 4), 0), ((4,), 1), ((3, 1, 7), 3), ((0,), 1)):
+        assert _rows(torch.zeros(*shape)).shape == (rows, shape[-1])
+
+
+@pytest.mark.gpu
+def test_rows_without_elements_are_refused():
+    from sesa import ops
+    from sesa._native import SesaError
+    i8 = lambda *s: torch.zeros(*s, dtype=torch.int8, device="cuda")  # noqa: E731
+    for bad in (lambda: ops.linear_i8(i8(2, 3, 0), torch.ones(2, 3, device="cuda"), i8(4, 0), torch.ones(4, device="cuda")),
+                lambda: ops.norm_residual(torch.zeros(2, 3, 0, device="cuda")), lambda: ops.quantize_i8(torch.zeros(2, 3, 0, device="cuda"))):
+        with pytest.raises(SesaError):
+            bad()
