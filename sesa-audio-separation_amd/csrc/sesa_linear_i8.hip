@@ -32,8 +32,11 @@ __device__ __forceinline__ i32x4 mfma_i8(i32x4 a, i32x4 b, i32x4 c) {
   return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
 }
 
-template <int ACT>
+// TO: fp32 results show what gelu_f's polynomial leaves (1.5e-7 of |v| / 2, more than the value itself below -5); 16-bit ones
+// do not, and their epilogue is bound by the VALU.
+template <int ACT, class TO>
 __device__ __forceinline__ float activate(float v) {
+  if constexpr (ACT == SESA_ACT_GELU && sizeof(TO) == 4) return gelu_fine_f(v);
   if constexpr (ACT == SESA_ACT_GELU) return gelu_f(v);
   if constexpr (ACT == SESA_ACT_TANH) return tanh_f(v);
   if constexpr (ACT == SESA_ACT_RELU) return v > 0.f || v != v ? v : 0.f;   // (keeps NaN)
@@ -248,7 +251,7 @@ __global__ void __launch_bounds__(WAN* WAM * 64, OCC) tile_kernel(LinArgs a) {
           const f32x4 b4 = *reinterpret_cast<const f32x4*>(b_l + c0 + 4 * j);
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            v[j >> 1][4 * (j & 1) + e] = activate<ACT>(fmaf((float)acc[u][j][i][e] * xs, w4[e], b4[e]));
+            v[j >> 1][4 * (j & 1) + e] = activate<ACT, TO>(fmaf((float)acc[u][j][i][e] * xs, w4[e], b4[e]));
         }
         if (m < a.m && left > 0) {
           TO* o = out + (int64_t)m * a.o_ld + n;
@@ -317,7 +320,7 @@ __global__ void __launch_bounds__(512) few_kernel(LinArgs a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (n + e < a.n)
-          out[(int64_t)m * a.o_ld + n + e] = (TO)activate<decltype(act)::value>(
+          out[(int64_t)m * a.o_ld + n + e] = (TO)activate<decltype(act)::value, TO>(
               fmaf((float)v[e] * xs, a.w_scale[n + e], a.bias ? a.bias[n + e] : 0.f));
     }
   });

@@ -104,6 +104,25 @@ __device__ __forceinline__ float gelu_f(float v) {
   return fmaf(-fminf(z, 1e30f), q, fmaxf(v, 0.f));   // (the minimum: an infinity times its tail of 0)
 }
 
+// The same to fp32: erfc(z) = t P7(t) exp(-z^2), t = 1 / (1 + 0.44 z), P fitted here to the least relative error on z in
+// [0, 10], 1.8e-7 (the 1 / 2 in the coefficients).  rms error on [-8, 8] 5.2e-8, which is the result's own rounding; three
+// operations more than gelu_f.
+__device__ __forceinline__ float gelu_fine_f(float v) {
+  const float z = fabsf(v);
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.44f * 0.70710678118654752440f, z, 1.0f));
+  float p = 0.0356115793f;
+  p = fmaf(p, t, -0.13897336f);
+  p = fmaf(p, t, 0.148342622f);
+  p = fmaf(p, t, -0.0100893122f);
+  p = fmaf(p, t, 0.107905584f);
+  p = fmaf(p, t, 0.108656933f);
+  p = fmaf(p, t, 0.124435566f);
+  p = fmaf(p, t, 0.124110478f);
+  const float w = v * 0.84932180028801904272f;
+  const float q = p * t * __builtin_amdgcn_exp2f(-(w * w));
+  return fmaf(-fminf(z, 1e30f), q, fmaxf(v, 0.f));
+}
+
 // Workgroup barrier behind this wave's own LDS operations that leaves loads to LDS in flight: __syncthreads() would wait
 // for all of them, whatever stage they are for.  A kernel that uses it waits on vmcnt for the stage it is about to read.
 __device__ __forceinline__ void stage_sync() {

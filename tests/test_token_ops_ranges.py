@@ -554,3 +554,24 @@ def test_rows_without_elements_are_refused():
                 lambda: ops.norm_residual(torch.zeros(2, 3, 0, device="cuda")), lambda: ops.quantize_i8(torch.zeros(2, 3, 0, device="cuda"))):
         with pytest.raises(SesaError):
             bad()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 40, 300])
+def test_linear_i8_gelu_in_fp32(m):
+    """fp32 results carry GELU to fp32, down its negative tail (the argument exact: one product by powers of two)."""
+    from sesa import ops
+    x = torch.arange(-128, 128, device="cuda").to(torch.int8)[:, None]
+    ws = torch.tensor([2.0 ** -4, 2.0 ** -5, 2.0 ** -9, 2.0 ** 3], device="cuda")
+    w = torch.ones(4, 1, dtype=torch.int8, device="cuda")
+    for at in range(0, 256, m):
+        rows = x[at:at + m]
+        got = ops.linear_i8(rows, torch.ones(len(rows), device="cuda"), w, ws, act="gelu", out_dtype=torch.float32).double()
+        v = rows.double() * ws.double()
+        ref = 0.5 * v * torch.erfc(-v / math.sqrt(2.0))
+        # erfc to 4 half-steps and two products; its argument half a step off counts |v|^2 times where erfc falls
+        tol = (8 + v * v) * 2.0 ** -23 * ref.abs() + 2.0 ** -140
+        assert bool(((got - ref).abs() <= tol).all()), float(((got - ref).abs() / tol).max())
+    big = torch.tensor([[-128], [127]], dtype=torch.int8, device="cuda")
+    y = ops.linear_i8(big, torch.full((2,), 3e38, device="cuda"), w[:1], torch.ones(1, device="cuda"), act="gelu", out_dtype=torch.float32)
+    assert float(y[0]) == 0 and float(y[1]) == math.inf
