@@ -155,23 +155,44 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) norm_residual_kernel(se
       if (e < left) top = max(top, __builtin_bit_cast(uint32_t, y[c][e]) & 0x7fffffffu);
   }
   top = row_max<TPR>(top, red + 64);
-  const float amax = __builtin_bit_cast(float, top);
+  float amax = __builtin_bit_cast(float, top), down = 1.f;
   const bool fine = top < 0x7f800000u, some = amax >= 1.6e-36f;   // (below: the scale would be subnormal; counts as 0)
-  const float scale = fine && some ? amax / 127.f : 0.f, inv = fine && some ? 1.f / scale : 0.f;
-  if (t == 0) a.q_scale[row] = fine ? scale : __builtin_nanf("");
+  // amax / 127 and 1 / scale, each rounded to nearest: an estimate and one correction by its exact remainder (Markstein).
+  float scale = 0.f, inv = 0.f;
+  if (fine && some) {
+    if (amax < 0x1p-90f) {   // (rare: the remainders would be subnormal)
+      amax *= 0x1p64f;
+      down = 0x1p-64f;
+#pragma unroll
+      for (int c = 0; c < NCH; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[c][e] *= 0x1p64f;
+    }
+    scale = amax * (1.f / 127.f);
+    scale = fmaf(fmaf(-127.f, scale, amax), 1.f / 127.f, scale);
+    inv = __builtin_amdgcn_rcpf(scale);
+    inv = fmaf(fmaf(-inv, scale, 1.f), inv, inv);
+  }
+  if (t == 0) a.q_scale[row] = fine ? scale * down : __builtin_nanf("");
 #pragma unroll
   for (int c = 0; c < NCH; ++c) {
     const int at = (c * TPR + t) * 8, left = dim - at;
     if (left <= 0) continue;
     int8_t* qp = a.q + row * a.q_ld + at;
-    uint32_t w[2] = {0, 0};
+    uint32_t w[2] = {0, 0};   // (a row without a scale stores 0)
+    if (inv > 0.f) {
+      uint32_t k[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      // The quotient y / scale rounded to nearest, as a division gives it, from the rounded reciprocal and one correction by
-      // the exact remainder (Markstein); at most 127 (1 + 2^-23) in size: no clamp needed; a row without a scale stores 0.
-      const float g = y[c][e] * inv;
-      const int k = inv > 0.f ? (int)rintf(fmaf(fmaf(-g, scale, y[c][e]), inv, g)) : 0;
-      w[e >> 2] |= (uint32_t)(k & 0xff) << (8 * (e & 3));
+      for (int e = 0; e < 8; ++e) {
+        // y / scale rounded to nearest, the same way; at most 127 (1 + 2^-23) in size: no clamp needed.  1.5 * 2^23 on top
+        // rounds it to a whole number, half to even, whose two's complement is the sum's low byte.
+        const float g = y[c][e] * inv;
+        k[e] = __builtin_bit_cast(uint32_t, fmaf(fmaf(-g, scale, y[c][e]), inv, g) + 12582912.f);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)   // the four low bytes: two and two, then all
+        w[h] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(k[4 * h + 3], k[4 * h + 2], 0x0c0c0400u),
+                                     __builtin_amdgcn_perm(k[4 * h + 1], k[4 * h], 0x0c0c0400u), 0x05040100u);
     }
     if (left >= 8) {
       struct __attribute__((packed)) B8 { uint32_t a, b; };

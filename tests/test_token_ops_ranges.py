@@ -175,7 +175,7 @@ def test_attention_one_large_score_over_many_small_ones(d, dt, n):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dt,rows,dim", [(torch.float32, 40_000, 512), (torch.float32, 3000, 1537), (torch.float16, 20_000, 1024),
                                          (torch.bfloat16, 500, 9000)])
-@pytest.mark.parametrize("size", [1.0, 1e-30, 1e30])
+@pytest.mark.parametrize("size", [1.0, 1e-35, 1e-30, 1e30, 5e37])
 def test_quantize_i8_is_the_rounded_quotient(dt, rows, dim, size):
     """q = round(x / q_scale) to even for every element, the quotient rounded once to fp32 (here: in 64 bits, which holds it
     well enough that rounding it again is the same)."""
