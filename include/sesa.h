@@ -328,7 +328,8 @@ int sesa_linear_i8(const int8_t* x, int64_t x_ld, const float* x_scale, const in
  *   y = residual + scale * gate_act(gate) * post_norm(x)        (the block's output joins the residual stream)
  *   n = pre_norm(y)                                              (the next block's input)
  * residual, scale, gate and the norms are optional; statistics and everything between the loads and the one
- * rounding of y and of n are fp32 (n comes from the unrounded y).  With q instead of n the rows leave in 8 bits:
+ * rounding of y and of n are fp32 (n comes from the unrounded y; a normalised row's sum of squares has to fit:
+ * elements up to about 1e19 / sqrt(dim)).  With q instead of n the rows leave in 8 bits:
  *   q_scale = max |n| / 127 over the row, q = round-half-even(n / q_scale)
  * (a row with nothing above 1.6e-36: scale 0, q 0; a row holding a NaN or an infinity: scale NaN, q 0).
  * y may be residual (same ld): in place.  No other operands may overlap.  dim <= 32768.

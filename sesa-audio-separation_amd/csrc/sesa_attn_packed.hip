@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(NW * 64, D == 64 ? (LOADS != kRegisters ? 4 : 
   for (int db = 0; db < D / 32; ++db)
 #pragma unroll
     for (int r = 0; r < 16; ++r) over = over || o[db][r] != o[db][r];
-  over = far || (over && l_run == l_run);
+  over = q_ok && (far || (over && l_run == l_run));
   const uint64_t redo = __ballot(over);
   if (redo) {
     // Rare, and bound by the latency of one key after the other, 2.4 us (12289 causal tokens, 32 / 8 heads x 128, bf16: 0.4

@@ -3,8 +3,8 @@
 // Memory bound: x, residual (and a per-row gate) are read once, y and n written once, and every value of a row stays
 // in registers between the reductions.  One wave per row up to dim 1024 (no LDS, no barrier), 256 threads up to 4096,
 // 1024 above: a thread keeps at most 32 values and enough rows are in flight to cover the loads (16384 x 8192 bf16,
-// sandwich norms and gate: 334 us at 256 threads, 278 at 512, 275 at 1024; 16384 x 4096: 134, 139, -).  Statistics are two-pass over the registers (mean, then squared deviations), so LayerNorm does not
-// cancel.
+// sandwich norms and gate: 334 us at 256 threads, 278 at 512, 275 at 1024; 16384 x 4096: 134, 139, -).  Statistics are
+// two-pass over the registers (mean, then squared deviations), so LayerNorm does not cancel.
 #include "sesa_tokens.hpp"
 
 namespace sesa {

@@ -108,7 +108,7 @@ def _launch(op, idx, entry, *args):
 _Tensor = torch.Tensor
 _PLAIN = {torch.Tensor, torch.nn.Parameter, type(None)}
 _compiling = torch.compiler.is_compiling
-_tracing = torch._C._get_tracing_state
+_tracing = torch._C._is_tracing
 _dispatch_modes = torch._C._len_torch_dispatch_stack
 _function_modes = torch._C._len_torch_function_stack
 _transforms = torch._C._are_functorch_transforms_active
@@ -121,7 +121,7 @@ def _plain(*tensors):
     """Whether nothing but the values counts: plain tensors (or None), and no torch.compile or torch.jit trace, no torch.func
     transform, no mode and no forward-mode level that would have to see the op."""
     return set(map(type, tensors)) <= _PLAIN and not (_compiling() or _dispatch_modes() or _function_modes() or _transforms() or
-                                                      _tracing() is not None or _forward_ad._current_level >= 0)
+                                                      _tracing() or _forward_ad._current_level >= 0)
 
 
 def _eager(op, t, *more):
