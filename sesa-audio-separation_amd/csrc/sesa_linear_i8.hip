@@ -3,7 +3,8 @@
 // v_mfma_i32_16x16x64_i8 with the weights as the first operand: a lane's accumulators are then consecutive output
 // channels of one token.  The sums are exact 32-bit integers; scales, bias and activation are fp32, one rounding.  The
 // token's scale goes to the sum first: the two scales' own product may leave the range of fp32 where the result does not.
-// Measured: one token, 4096 -> 16384 (64 MB of weights) 17.1 us, 3.9 TB/s; 8192 tokens 482 us, 2.28 POP/s.
+// Measured: one token, 4096 -> 16384 (64 MB of weights) 17.2 us, 3.9 TB/s; 8192 tokens 485 us, 2.27 POP/s (542 us back to
+// back on the same inputs: the clock sinks).
 //
 // Two kernels:
 //  * tile_kernel: BM tokens x BN channels per workgroup, K in 128-byte steps through a ring of LDS stages.

@@ -3,7 +3,7 @@
 // Memory bound (each element read once and written once).  A thread owns up to 8 pairs of one token (16-byte loads and
 // stores of 16-bit types), takes their sines and cosines once and applies them to its share of the heads of every tensor;
 // heads are dealt to more threads only where the tokens alone do not fill the chip.  24001 tokens, 32 + 8 heads x 128,
-// bf16: 108 us, 4.5 TB/s of the copy's 5.1; three tokens: 5.4 us on the device.
+// bf16: 109 us, 4.5 TB/s of the copy's 5.1; three tokens: 5.6 us on the device.
 // Angle: one turn is 2^64.  freqs / (2 pi), with 1 / (2 pi) in two doubles, is reduced to a fraction of a turn and held as
 // a 64-bit integer, so position * freq wraps modulo one turn in integer arithmetic: the phase is off by at most |position|
 // 2^-63 turns for |freq| up to 2^40 (one double: |position| max(1, |freq| / pi) 2^-54; an fp32 product is off by half a
