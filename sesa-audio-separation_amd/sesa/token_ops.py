@@ -398,6 +398,12 @@ def _(xs, positions, freqs, sections, layout):
 
 @_define("rope_axes_(Tensor(a!)[] xs, Tensor positions, Tensor freqs, int[] sections, str layout) -> ()")
 def _rope_axes_(xs, positions, freqs, sections, layout):
+    _rope_places(xs)
+    _rope_call("rope_axes_", xs, xs, positions, freqs, sections, layout)
+    _written(xs)
+
+
+def _rope_places(xs):
     if not 1 <= len(xs) <= 2:
         _fail("rope_axes_", f"one or two tensors, got {len(xs)}")
     for x in xs:
@@ -407,8 +413,6 @@ def _rope_axes_(xs, positions, freqs, sections, layout):
                                 f"dimension; got {list(x.shape)} with strides {list(x.stride())}")
     if len(xs) == 2 and not _apart(*xs):
         _fail("rope_axes_", "the two tensors overlap")
-    _rope_call("rope_axes_", xs, xs, positions, freqs, sections, layout)
-    _written(xs)
 
 
 @torch.library.register_fake("sesa::rope_axes_", lib=_LIB)
@@ -540,8 +544,15 @@ def rope_axes(q, k, positions, freqs, sections, *, layout="halves"):
 
 def rope_axes_(q, k, positions, freqs, sections, *, layout="halves"):
     """``rope_axes`` in place on q and k (k may be None)."""
-    call = _rope_axes_ if _eager("rope_axes_", q, k, positions, freqs) else torch.ops.sesa.rope_axes_
-    call([q] if k is None else [q, k], positions, freqs, sections, layout)
+    eager = _eager("rope_axes_", q, k, positions, freqs)
+    xs = [q] if k is None else [q, k]
+    if _tracing():   # (torch.jit drops an op that only writes a list of tensors)
+        _rope_places(xs)
+        for x, y in zip(xs, torch.ops.sesa.rope_axes(xs, positions, freqs, sections, layout)):
+            x.copy_(y)
+        return
+    call = _rope_axes_ if eager else torch.ops.sesa.rope_axes_
+    call(xs, positions, freqs, sections, layout)
 
 
 def attention_packed(q, k, v, cu_seqlens=None, *, causal=True, scale=None, gate=None, out=None):

@@ -575,3 +575,47 @@ def test_linear_i8_gelu_in_fp32(m):
     big = torch.tensor([[-128], [127]], dtype=torch.int8, device="cuda")
     y = ops.linear_i8(big, torch.full((2,), 3e38, device="cuda"), w[:1], torch.ones(1, device="cuda"), act="gelu", out_dtype=torch.float32)
     assert float(y[0]) == 0 and float(y[1]) == math.inf
+
+
+@pytest.mark.gpu
+def test_jit_trace_of_calls_in_place(some):
+    """In-place rotation and attention into a given tensor, traced: the traced function does the same to new inputs."""
+    from sesa import ops
+
+    def f(qkv, pos, freqs):
+        rows = qkv * 1
+        q, k, v = rows.split([2, 1, 1], 1)
+        ops.rope_axes_(q, k, pos, freqs, [8])
+        out = torch.zeros_like(q)
+        ops.attention_packed(q, k, v, out=out)
+        return rows, out
+    names = ("qkv", "pos", "freqs")
+    traced = torch.jit.trace(f, tuple(some(1)[n] for n in names), check_trace=False)
+    for seed in (2, 3):
+        args = [some(seed)[n] for n in names]
+        for a, b in zip(traced(*args), f(*args)):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_calls_from_several_threads(some):
+    """Two threads, each with its own stream and inputs, at once."""
+    import threading
+    sets = [some(s) for s in (11, 12)]
+    want = [[t.clone() for t in all_ops(**s)] for s in sets]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                got = all_ops(**sets[i])
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                    wrong.append(i)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong

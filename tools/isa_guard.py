@@ -1,10 +1,9 @@
 """Build guard: fail if libsesa's gfx950 code contains a packed-fp32 VALU instruction.
 
-Round 6 finding (profiles/r06_pk_opsel_hazard.txt): on MI355X, v_pk_add_f32 / v_pk_mul_f32 (/ fma) whose
-op_sel picks the high half of a source for the low result -- the form the SLP vectorizer emits for complex
-arithmetic -- return wrong values while another wave on the same CU is executing MFMAs (tools/victim_stress.py
-form2 / form3: 4-6 of 40 chained runs corrupted; the same chain without op_sel, 0 of 40).  That was the cross-stream
-discrepancy of rounds 4-5: the FFT kernels (STFT / iSTFT) computed wrong columns whenever another stream's MFMA
+On MI355X, v_pk_add_f32 / v_pk_mul_f32 (/ fma) whose op_sel picks the high half of a source for the low result -- the form
+the SLP vectorizer emits for complex arithmetic -- return wrong values while another wave on the same CU is executing
+MFMAs (tools/victim_stress.py form2 / form3: 4-6 of 40 chained runs corrupted; the same chain without op_sel, 0 of 40;
+profiles/r06_pk_opsel_hazard.txt): the FFT kernels (STFT / iSTFT) computed wrong columns whenever another stream's MFMA
 kernel shared their CUs.  The compiler picks the form by itself wherever it packs, so libsesa is built without the packed
 fp32 feature (csrc/Makefile); this check keeps it that way.
 
