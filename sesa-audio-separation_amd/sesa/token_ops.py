@@ -546,7 +546,7 @@ def rope_axes_(q, k, positions, freqs, sections, *, layout="halves"):
     """``rope_axes`` in place on q and k (k may be None)."""
     eager = _eager("rope_axes_", q, k, positions, freqs)
     xs = [q] if k is None else [q, k]
-    if _tracing():   # (torch.jit drops an op that only writes a list of tensors)
+    if not eager and not _compiling() and _tracing():   # (torch.jit drops an op that only writes a list of tensors)
         _rope_places(xs)
         for x, y in zip(xs, torch.ops.sesa.rope_axes(xs, positions, freqs, sections, layout)):
             x.copy_(y)

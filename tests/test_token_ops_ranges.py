@@ -619,3 +619,25 @@ def test_calls_from_several_threads(some):
     for t in threads:
         t.join()
     assert not wrong
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("backend", ["eager", "aot_eager"])
+def test_compiled_calls_in_place(some, backend):
+    """In-place rotation and attention into a given tensor in a compiled function, inputs of two sizes."""
+    from sesa import ops
+
+    def f(qkv, pos, freqs):
+        rows = qkv * 1
+        q, k, v = rows[:, :2], rows[:, 2:3], rows[:, 3:]
+        ops.rope_axes_(q, k, pos, freqs, [8])
+        out = torch.zeros(rows.shape[0], 2, 16, device="cuda", dtype=torch.float16)
+        ops.attention_packed(q, k, v, out=out)
+        return rows, out
+    torch._dynamo.reset()
+    compiled = torch.compile(f, backend=backend, fullgraph=True)
+    for seed, n in ((2, 6), (3, 6), (4, 5)):
+        s = some(seed)
+        args = (s["qkv"][:n], s["pos"][:n], s["freqs"])
+        for a, b in zip(compiled(*args), f(*args)):
+            assert torch.equal(a, b)
