@@ -409,9 +409,8 @@ int sesa_rope_axes(const sesa_rope_args* args, void* stream);
  * head_dim a multiple of 8, 8..128; heads a multiple of kv_heads; fp16 or bf16.  Scores, softmax statistics and
  * sums fp32; the probabilities are rounded once to the type for the product with v.  A masked key contributes
  * nothing, whatever its k and v hold; a visible infinite v with a finite score counts however small its probability.
- * Rows that meet an infinite or NaN v under a probability of 0 (a masked key's in the same 64 keys included) and rows
- * with scores beyond 2.9e6 are done over key by key: the same answer, 30 to 170 times as long where every tile has
- * such rows.  out may not overlap the inputs.
+ * Tiles whose rows meet an infinite or NaN v (a masked key's in the same 64 keys included) or scores beyond 2.9e6 go
+ * through their keys a second time: about three times as long.  out may not overlap the inputs.
  */
 typedef struct sesa_attn_args {
   int64_t tokens;

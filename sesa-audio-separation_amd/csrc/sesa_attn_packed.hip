@@ -72,6 +72,7 @@ __global__ void __launch_bounds__(NW * 64, D == 64 ? (LOADS != kRegisters ? 4 : 
   constexpr int BQ = NW * 32, NTH = NW * 64, ROW = D * 2, IMG = kKeys * ROW, CH = D / 8, IT = kKeys * CH / NTH;
   constexpr float kLog2e = 1.4426950408889634f;
   __shared__ __attribute__((aligned(16))) char smem[4 * IMG];   // [stage][K, V], rows of D elements
+  __shared__ int again;                                         // a row of the tile has to be done over
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, hl = lane >> 5;
   const int group = a.heads / a.kv_heads;
@@ -94,6 +95,7 @@ __global__ void __launch_bounds__(NW * 64, D == 64 ? (LOADS != kRegisters ? 4 : 
       for (int d = 8 * hl; d < a.head_dim; d += 16) store16(out + d, u32x4{0u, 0u, 0u, 0u});
     return;
   }
+  if (tid == 0) again = 0;   // (set behind the barriers of the pass)
   const int hd = a.head_dim;
   const T* kp = reinterpret_cast<const T*>(a.k) + ln * a.k_l + kh * a.k_h;
   const T* vp = reinterpret_cast<const T*>(a.v) + ln * a.v_l + kh * a.v_h;
@@ -112,10 +114,11 @@ __global__ void __launch_bounds__(NW * 64, D == 64 ? (LOADS != kRegisters ? 4 : 
   for (int db = 0; db < D / 32; ++db)
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[db][r] = 0.f;
-  // Running reference r_run = a largest score so far times c (less kLift), rounded to fp32, and the running sum.  Every probability is
-  // exp2(s c - r_run) with the product unrounded: the reference's own rounding is in all of them alike and cancels (a
+  // Running reference r_run = a largest score so far times c (less kLift), rounded to fp32, and the running sum.  Every
+  // probability is exp2(s c - r_run) with the product unrounded: the reference's own rounding is in all of them alike and cancels (a
   // product rounded anew for each use would not: 6e-2 of a block's weight at scores of 1e6).  From kFar on that rounding
-  // may reach a factor of 2^0.5 and, further out, the range of P, so such rows are done over below.
+  // may reach a factor of 2^0.5 and, further out, the range of P, so such rows are done over, where `sub` takes the maximum
+  // off before the scaling: exactly 0 at the largest score, whatever its size.
   // kLift: fp16 takes P 2^7 higher, so that it is normal down to 2^-21 of the largest where plain P ends at 2^-14 (below,
   // a step is 2^-24: 100000 keys at 1.5 steps each lost a third of their weight).
   constexpr float kLift = std::is_same<T, f16>::value ? 7.f : 0.f;
@@ -212,8 +215,36 @@ __global__ void __launch_bounds__(NW * 64, D == 64 ? (LOADS != kRegisters ? 4 : 
   // blocks all of whose keys every query of the tile sees
   const int n_whole = (min(end, a.causal ? q0 + 1 : end) - start) / kKeys;
 
-  auto step = [&](int kb, auto masked) {
-    constexpr bool MASKED = decltype(masked)::value;
+  // Second pass (REDO): infinite and NaN elements of v are taken out, so that a probability of 0 -- a key that the row does
+  // not see, or one too small for the type -- times one of them is no NaN, and come back as what the keys that the row does
+  // see make of them.  code: 1 for +inf, 128 for -inf, 16384 for NaN; 16 keys' codes add up without a carry.
+  auto take_out = [](u32x4& v, u32x4& code) {
+    constexpr bool F16 = std::is_same<T, f16>::value;
+    constexpr uint32_t kExp = F16 ? 0x7c00 : 0x7f80, kFrac = F16 ? 0x03ff : 0x007f;
+    constexpr uint32_t kPos = F16 ? 0x3c00 : 0x3f80, kNeg = F16 ? 0x5800 : 0x4300, kNan = F16 ? 0x7400 : 0x4680;
+    bool any = false;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      uint32_t keep = 0, out = 0;
+#pragma unroll
+      for (int h = 0; h < 32; h += 16) {
+        const uint32_t e = v[q] >> h & 0xffffu;
+        const bool bad = (e & kExp) == kExp;
+        any = any || bad;
+        keep |= (bad ? 0u : e) << h;
+        out |= (!bad ? 0u : e & kFrac ? kNan : e >> 15 ? kNeg : kPos) << h;
+      }
+      v[q] = keep;
+      code[q] = out;
+    }
+    return any;
+  };
+  // A finite score never weighs less than this in the second pass, nor does a rescaling: too little to move a finite sum; an
+  // infinite one stays what it is, and p > 0 says which keys the row sees.
+  constexpr float kLeast = 1.17549435e-38f;   // 2^-126
+
+  auto step = [&](int kb, auto masked, auto second) {
+    constexpr bool MASKED = decltype(masked)::value, REDO = decltype(second)::value;
     const int cur = (kb & 1) * 2 * IMG, next = ((kb + 1) & 1) * 2 * IMG;
     // this wave's part of block kb has landed; behind the barrier everyone's has, and everyone is done with block
     // kb - 1, whose place block kb + 1 takes
@@ -249,10 +280,12 @@ __global__ void __launch_bounds__(NW * 64, D == 64 ? (LOADS != kRegisters ? 4 : 
     top = max_halves(top);
     // The reference moves only when a block exceeds it by more than 2^8 in the exponential (P stays below 2^(8.5 + kLift), in
     // range for fp16), so most blocks leave O alone.  Both halves of a query hold the same values, so they agree.
-    if (fmaf(top, c, -r_run) > 8.f + kLift) {
-      const float r = fmaf(top, c, -kLift);
-      const float alpha = __builtin_amdgcn_exp2f(r_run - r);   // (the first time: 0)
-      far = far || (fabsf(top) < INFINITY && !(fabsf(r) <= kFar));
+    const bool raw = REDO && far;   // r_run holds the score itself
+    if ((raw ? (top - r_run) * c + kLift : fmaf(top, c, -r_run)) > 8.f + kLift) {
+      const float r = raw ? top : fmaf(top, c, -kLift);
+      float alpha = __builtin_amdgcn_exp2f(raw ? (r_run - r) * c : r_run - r);   // (the first time: 0)
+      if constexpr (REDO) alpha = fmaxf(alpha, kLeast);
+      else far = far || (fabsf(top) < INFINITY && !(fabsf(r) <= kFar));
       l_run *= alpha;
 #pragma unroll
       for (int db = 0; db < D / 32; ++db)
@@ -260,13 +293,15 @@ __global__ void __launch_bounds__(NW * 64, D == 64 ? (LOADS != kRegisters ? 4 : 
         for (int r = 0; r < 16; ++r) o[db][r] *= alpha;
       r_run = r;
     }
-    const float rc = r_run == -INFINITY ? 0.f : r_run;   // (no finite score so far: every P is exp(-inf) = 0)
+    float rc = r_run == -INFINITY ? 0.f : r_run, sub = 0.f;   // (no finite score so far: every P is exp(-inf) = 0)
+    if (raw) sub = rc, rc = -kLift;
     float sum[2] = {0.f, 0.f};   // a block's own first: small ones would be lost one by one against a large l_run
 #pragma unroll
     for (int rb = 0; rb < 2; ++rb)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(s[rb][r], c, -rc));
+        float p = __builtin_amdgcn_exp2f(fmaf(REDO ? s[rb][r] - sub : s[rb][r], c, -rc));
+        if (REDO && p < kLeast && s[rb][r] > -INFINITY) p = kLeast;
         s[rb][r] = p;
         sum[rb] += p;
       }
@@ -280,6 +315,26 @@ __global__ void __launch_bounds__(NW * 64, D == 64 ? (LOADS != kRegisters ? 4 : 
       u32x4 vf[D / 32];
 #pragma unroll
       for (int db = 0; db < D / 32; ++db) vf[db] = vt(cur, ks, db);
+      if constexpr (REDO) {
+        u32x4 seen;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) seen[q] = pack2t<T>(sv[r0 + 2 * q] > 0.f ? 1.f : 0.f, sv[r0 + 2 * q + 1] > 0.f ? 1.f : 0.f);
+#pragma unroll
+        for (int db = 0; db < D / 32; ++db) {
+          u32x4 code;
+          if (__ballot(take_out(vf[db], code))) {
+            f32x16 n;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) n[r] = 0.f;
+            n = mfma16<T>(code, seen, n);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int k = (int)n[r];
+              o[db][r] += (k >= 16384 ? __builtin_nanf("") : 0.f) + ((k & 16383) >= 128 ? -INFINITY : 0.f) + (k & 127 ? INFINITY : 0.f);
+            }
+          }
+        }
+      }
 #pragma unroll
       for (int db = 0; db < D / 32; ++db) o[db] = mfma16<T>(vf[db], pf, o[db]);
     }
@@ -297,70 +352,36 @@ __global__ void __launch_bounds__(NW * 64, D == 64 ? (LOADS != kRegisters ? 4 : 
   store_block(0);
   __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0), where the compiler sees it: no wait for Q inside the loop
   int kb = 0;
-  for (; kb < n_whole; ++kb) step(kb, std::false_type{});
-  for (; kb < n_blocks; ++kb) step(kb, std::true_type{});
+  for (; kb < n_whole; ++kb) step(kb, std::false_type{}, std::false_type{});
+  for (; kb < n_blocks; ++kb) step(kb, std::true_type{}, std::false_type{});
   l_run += __shfl_xor(l_run, 32);
 
-  // Rows to do over: `far`, and NaN in o under finite probabilities.  A probability of 0 -- a key that the row does not see,
-  // or one too small for the type -- times an infinite or NaN v is NaN, and so is an infinity times a rescaling by 0.
-  // (NaN scores make the sum NaN as well: that row is NaN by the formula.)  Nothing to look for inside the loop.
+  // Rows to do over: `far`, and NaN in o under finite probabilities (0 times an infinite or NaN v, an infinity times a
+  // rescaling by 0; NaN scores make the sum NaN as well: that row is NaN by the formula).  Nothing to look for inside the
+  // loop.  The whole tile goes through its keys once more, with the elements taken out (2 x 801 tokens x 62 lanes, every tile:
+  // 267 -> 734 us; 12289 causal tokens, scores of 1e9 in every row: 0.4 -> 1.3 ms; a serial pass over a row's keys instead
+  // took 10 and 69 ms); rows that did not ask for it come out as they were.
   bool over = false;
 #pragma unroll
   for (int db = 0; db < D / 32; ++db)
 #pragma unroll
     for (int r = 0; r < 16; ++r) over = over || o[db][r] != o[db][r];
   over = q_ok && (far || (over && l_run == l_run));
-  const uint64_t redo = __ballot(over);
-  if (redo) {
-    // Rare, and bound by the latency of one key after the other, 2.4 us (12289 causal tokens, 32 / 8 heads x 128, bf16: 0.4
-    // ms; NaN in the last token 30 ms, scores of 1e9 in every row 69 ms): those rows key by key, each only with the keys
-    // it sees, from global memory and without matrix instructions (no barrier: the waves of the tile may differ); the
-    // wave's other rows keep what they have.  A lane half has its half of q's and o's elements.  The maximum is taken off
-    // before the scaling: exactly 0 at the largest score, whatever its size.  A finite score never weighs less than
-    // kLeast, nor does a rescaling: too little to move a finite sum, and an infinite v stays what it is.
-    constexpr float kLeast = 1.17549435e-38f;   // 2^-126
-    const bool mine = ((uint32_t)(redo >> 32) | (uint32_t)redo) >> l32 & 1;
-    const int64_t lim = min((int64_t)(end - 1), a.causal ? q_pos : (int64_t)(end - 1));
-    float m_run = -INFINITY;
-    if (mine) {
-      l_run = 0.f;
+  if (__ballot(over) && lane == 0) again = 1;
+  sesa_sync();
+  if (__builtin_amdgcn_readfirstlane(again)) {
+    r_run = -INFINITY;
+    l_run = 0.f;
 #pragma unroll
-      for (int db = 0; db < D / 32; ++db)
+    for (int db = 0; db < D / 32; ++db)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) o[db][r] = 0.f;
-    }
+      for (int r = 0; r < 16; ++r) o[db][r] = 0.f;
+    if constexpr (DMA) offsets(min(kKeys, end - start));
+    load_block(0, 0);
+    store_block(0);
 #pragma unroll 1
-    for (int64_t j = start; j < last; ++j) {
-      const T* kj = kp + j * a.k_t;
-      const T* vj = vp + j * a.v_t;
-      float dot = 0.f;
-#pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) {
-        float kv[8];
-        load8(kj + 16 * ks + 8 * hl, hd - 16 * ks - 8 * hl, kv);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint32_t w = qf[ks][e >> 1];
-          dot = fmaf((float)__builtin_bit_cast(T, (uint16_t)(e & 1 ? w >> 16 : w & 0xffffu)), kv[e], dot);
-        }
-      }
-      dot += __shfl_xor(dot, 32);
-      if (j > lim || !mine) continue;
-      const float top = fmaxf(m_run, dot);
-      const float base = top == -INFINITY ? 0.f : top;
-      const float alpha = fmaxf(__builtin_amdgcn_exp2f((m_run - base) * c), kLeast);
-      float p = __builtin_amdgcn_exp2f((dot - base) * c);
-      if (p < kLeast && dot > -INFINITY) p = kLeast;
-      m_run = top;
-      l_run = fmaf(l_run, alpha, p);
-#pragma unroll
-      for (int db = 0; db < D / 32; ++db)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int d = db * 32 + 8 * (r >> 2) + 4 * hl + (r & 3);
-          o[db][r] = fmaf(p, d < hd ? (float)vj[d] : 0.f, o[db][r] * alpha);
-        }
-    }
+    for (kb = 0; kb < n_blocks; ++kb) step(kb, std::true_type{}, std::true_type{});
+    l_run += __shfl_xor(l_run, 32);
   }
 
   if (!q_ok) return;

@@ -641,3 +641,66 @@ def test_compiled_calls_in_place(some, backend):
         args = (s["qkv"][:n], s["pos"][:n], s["freqs"])
         for a, b in zip(compiled(*args), f(*args)):
             assert torch.equal(a, b)
+
+
+# ---- attention_packed: the second pass -------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("d,dt", [(64, "f16"), (64, "bf16"), (128, "f16"), (128, "bf16"), (40, "f16"), (96, "bf16")])
+@pytest.mark.parametrize("odd", [False, True])
+def test_attention_second_pass_leaves_finite_columns_alone(d, dt, causal, odd):
+    """A tile that goes through its keys twice: the columns without non-finite values, and the rows that did not ask for it,
+    bit for bit what they are without; infinities of both signs and NaN meet in a column as in the formula."""
+    from sesa import ops
+    cu, cut = cu_of([700, 333])
+    g = gen(d)
+    pad = (lambda x: torch.nn.functional.pad(x, (1, 2))[..., 1:d + 1]) if odd else (lambda x: x)
+    q, k, v = (torch.randn(1033, n, d, generator=g, device="cuda").to(DT[dt]) for n in (4, 2, 2))
+    bad = {2: (7, math.inf), 5: (7, -math.inf), 11: (40, math.nan), 17: (699, math.inf), 19: (1032, math.nan), 23: (700, -math.inf)}
+    zero = v.clone()
+    for col, (key, val) in bad.items():
+        zero[key, 0, col], v[key, 0, col] = 0, val
+    zero[20:300, 0, 30], v[20:300, 0, 30] = 0, math.inf          # many at once, one sign ...
+    zero[50, 0, 31], v[50, 0, 31] = 0, math.inf                  # ... and both in one column
+    zero[90, 0, 31], v[90, 0, 31] = 0, -math.inf
+    want = ops.attention_packed(*map(pad, (q, k, zero)), cut, causal=causal)
+    got = ops.attention_packed(*map(pad, (q, k, v)), cut, causal=causal)
+    assert torch.equal(got[:, 2:], want[:, 2:])                  # the other key head's
+    keep = [c for c in range(d) if c not in bad and c not in (30, 31)]
+    assert torch.equal(got[..., keep], want[..., keep])
+    row = torch.arange(1033, device="cuda")
+    for col, (key, val) in list(bad.items()) + [(30, (20, math.inf)), (31, (50, math.inf))]:
+        first = key < 700
+        sees = (row >= key if causal else row >= 0) & ((row < 700) == first)
+        seen, rest = got[:, :2, col][sees].float(), got[:, :2, col][~sees]
+        if col == 31:
+            both = got[:, :2, col][(row >= 90 if causal else row >= 0) & (row < 700)]
+            assert bool(torch.isnan(both).all())
+            if causal:
+                assert bool((got[50:90, :2, col] == math.inf).all())
+        else:
+            assert bool((torch.isnan(seen) if math.isnan(val) else seen == val).all())
+        assert torch.equal(rest, want[:, :2, col][~sees])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,dt", [(64, "f16"), (128, "bf16"), (48, "bf16")])
+def test_attention_far_rows_leave_the_others_alone(d, dt):
+    """One query of a tile with scores far out: its own row is done over, the tile's others keep their bits."""
+    from sesa import ops
+    q, k, v = (torch.randn(300, 1, d, generator=gen(d), device="cuda").to(DT[dt]) for _ in range(3))
+    want = ops.attention_packed(q, k, v)
+    q2 = q.clone()
+    q2[[131, 200]] = (q2[[131, 200]].float() * 6e3).to(DT[dt])
+    k2 = k.clone()
+    k2[:, :, 0] = (k2[:, :, 0].float() * 6e3).to(DT[dt])
+    q[:, :, 0], q2[:, :, 0] = 0, torch.where(torch.isin(torch.arange(300, device="cuda"), torch.tensor([131, 200], device="cuda"))[:, None], 6e3, 0.0)
+    want, got = ops.attention_packed(q, k2, v), ops.attention_packed(q2, k2, v)
+    near = [i for i in range(300) if i not in (131, 200)]
+    assert torch.equal(got[near], want[near])
+    for i in (131, 200):
+        s = (q2[i, 0].double() * k2[:i + 1, 0].double()).sum(-1)
+        top, at = s.topk(2)
+        # the two scores' sums of d products in fp32, d + 8 half-steps each, and e^-100 between them
+        assert float(top[0] - top[1]) > 2 * (d + 8) * 2.0 ** -24 * float(s.abs().max()) + 100 * d ** 0.5
+        assert torch.equal(got[i, 0], v[at[0], 0])
