@@ -9,9 +9,9 @@
 // four take 311, head 128 412 and 381), two waves read K and V from LDS for half the queries (501 at head 128).
 // Bound by the VALU about as much as by the matrix pipe: a 32 x 64 block is 32 exponentials and ~120 other operations
 // a lane (~1000 cycles) against 512 (head 64) or 1024 (head 128) cycles of products.  Measured: 12289 causal tokens,
-// 32 / 8 heads x 128, bf16 366-421 us by the sequences' lengths (0.92-1.05 PFLOP/s of its pairs; MFMA 54 % and VALU 52 %
+// 32 / 8 heads x 128, bf16 366-421 us by the sequences' lengths (0.92-1.05 PFLOP/s of its pairs; MFMA 53 % and VALU 52 %
 // busy); 2 x 801 tokens x 62 lanes, 8 heads x 64, fp16 267-271 us (0.61 PFLOP/s: 13 blocks a tile, one of them masked, 89 %
-// of the query rows used; MFMA 39 %, VALU 73 %).
+// of the query rows used; MFMA 40 %, VALU 74 %).
 // Probabilities are rounded to the 16-bit type for the product with v, which the matrix instructions take no wider: with the
 // result's own rounding 2.9e-4 of it in fp16 and 2.0e-3 in bf16 against 64 bits (2.1e-4 and 1.6e-3 without).
 #include "sesa_tokens.hpp"
@@ -406,7 +406,7 @@ int launch_attn(const sesa_attn_args& a, hipStream_t st) {
   const int64_t blocks = n_slots * a.heads * a.lanes;
   SESA_REQUIRE(blocks < (1ll << 31), SESA_ERR_INVALID, "attention_packed: too many tokens x heads x lanes");
   // 16-byte rows, and a block's byte offsets in 32 bits (12289 causal tokens, 32 / 8 heads, bf16, aligned | through registers:
-  // 64 181 | 220 us, 96 283 | 357, 128 294 | 395).  Rows of the whole tile width have a kernel of their own: the part rows'
+  // 64 181 | 224 us, 96 286 | 361, 128 298 | 400).  Rows of the whole tile width have a kernel of their own: the part rows'
   // masks take 4 % there.
   const int64_t strides = a.k_t | a.k_l | a.k_h | a.v_t | a.v_l | a.v_h;
   const bool dma = strides % 8 == 0 && ((uintptr_t)a.k | (uintptr_t)a.v) % 16 == 0 && a.k_t >= 0 && a.v_t >= 0 &&
