@@ -408,7 +408,8 @@ int sesa_rope_axes(const sesa_rope_args* args, void* stream);
  * they were, or set to 0 with zero_rest.  `lanes` runs of the same lengths lie side by side (strides *_l).
  * head_dim a multiple of 8, 8..128; heads a multiple of kv_heads; fp16 or bf16.  Scores, softmax statistics and
  * sums fp32; the probabilities are rounded once to the type for the product with v.  A masked key contributes
- * nothing, whatever its k and v hold; a visible infinite v with a finite score counts however small its probability.
+ * nothing, whatever its k and v hold, and so does one whose score is -inf; a visible infinite v with a finite score
+ * counts however small its probability.
  * Tiles whose rows meet an infinite or NaN v (a masked key's in the same 64 keys included) or scores beyond 2.9e6 go
  * through their keys a second time: about three times as long.  out may not overlap the inputs.
  */

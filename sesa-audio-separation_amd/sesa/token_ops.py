@@ -563,9 +563,10 @@ def attention_packed(q, k, v, cu_seqlens=None, *, causal=True, scale=None, gate=
     runs that many columns of the same lengths side by side (a Roformer's bands in its time attention).
     cu_seqlens int32 [sequences + 1] on the device, non-decreasing: sequence s is tokens cu_seqlens[s] ..
     cu_seqlens[s + 1] - 1 (None: one sequence).  It is read by the kernel and held to the run there: a boundary outside
-    is taken as the run's end, and boundaries out of order give unspecified rows, never an access outside.  gate: logits [tokens, (lanes,) heads], a sigmoid on each head's output.  scale: head_dim ** -0.5.
-    Rows of no sequence (behind the last) come back 0; with ``out`` they are left as they were.  Infinite or NaN values
-    and scores beyond 2.9e6 give what the formula says, in about three times the time."""
+    is taken as the run's end, and boundaries out of order give unspecified rows, never an access outside.  gate: logits
+    [tokens, (lanes,) heads], a sigmoid on each head's output.  scale: head_dim ** -0.5.  Rows of no sequence (behind the
+    last) come back 0; with ``out`` they are left as they were.  Infinite or NaN values and scores beyond 2.9e6 give what
+    the formula says (a key whose score is -inf: nothing), in about three times the time."""
     eager = _eager("attention_packed", q, k, v, cu_seqlens, gate, out)
     if out is None:
         call = _attention_packed if eager else torch.ops.sesa.attention_packed

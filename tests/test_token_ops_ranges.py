@@ -704,3 +704,21 @@ def test_attention_far_rows_leave_the_others_alone(d, dt):
         # the two scores' sums of d products in fp32, d + 8 half-steps each, and e^-100 between them
         assert float(top[0] - top[1]) > 2 * (d + 8) * 2.0 ** -24 * float(s.abs().max()) + 100 * d ** 0.5
         assert torch.equal(got[i, 0], v[at[0], 0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,dt", [(64, "f16"), (128, "bf16")])
+def test_attention_keys_with_a_score_of_minus_infinity(d, dt):
+    """A key whose score is -inf contributes nothing, whatever its value; a row of such keys alone is NaN."""
+    from sesa import ops
+    cu, cut = cu_of([150])
+    q, k, v = (torch.randn(150, 1, d, generator=gen(d), device="cuda").to(DT[dt]) for _ in range(3))
+    q[..., 0] = q[..., 0].abs() + 0.1
+    k[[0, 40, 100], :, 0] = -math.inf
+    rest = [i for i in range(150) if i not in (0, 40, 100)]
+    want = ops.attention_packed(q[rest], k[rest], v[rest])
+    for val in (1.0, math.inf, math.nan):
+        v[[0, 40, 100]] = val
+        got = ops.attention_packed(q, k, v, cut)
+        assert bool(torch.isnan(got[0]).all())
+        close(got[rest], want.double(), 4 * HALF[v.dtype] * v[rest].double().abs().amax())
